@@ -184,6 +184,48 @@ int32_t b2q_rms_norm_quantize_fp8_bf16(b2q_handle h, const void* x_bf16, void* r
                                        int64_t rows, int64_t cols, float eps, int fmt, int rounding, float* scales,
                                        uint8_t* codes, void* y_out_bf16);
 
+/* ---- FP8 with a scale for each block of 128: no counterpart in the reference, whose FP8 scales go per tensor.  Activations carry
+ * one f32 scale per (row, 128 columns), [rows x ceil(cols / 128)] row-major; weights one per 128 x 128 block,
+ * [ceil(N / 128) x ceil(K / 128)].  The last block of a row or column may be short. ---- */
+/* b2q_rms_norm_quantize_fp8_bf16 with that scale rule: scale = absmax(y)/max_val per block of 128 columns (1 for a block of
+ * zeros, never below 2^-126), code = encode(y/scale).  residual (optional) is updated in place and normalised; y_out (optional)
+ * receives bf16(y).  A row that holds a NaN, or whose sum of squares is infinite, gives what the formula gives (NaN, or zeros and
+ * NaN); its absmax is taken of the values that are not NaN. */
+int32_t b2q_rms_norm_quantize_fp8_block128_bf16(b2q_handle h, const void* x_bf16, void* residual_bf16, const void* gamma_bf16,
+                                                int64_t rows, int64_t cols, float eps, int fmt, int rounding, float* scales,
+                                                uint8_t* codes, void* y_out_bf16);
+/* b2q_swiglu_quantize_rows_bf16 with that scale rule: h = silu(gate) * up in f32, quantized per block of 128 columns. */
+int32_t b2q_swiglu_quantize_fp8_block128_bf16(b2q_handle h, const void* gate, const void* up, int64_t rows, int64_t cols,
+                                              int64_t ld, int fmt, int rounding, float* scales, uint8_t* codes);
+
+/* ---- paged KV cache in 8 bits with a scale for each page and head.  The reference quantizes a token at a time
+ * (crates/oxicuda-infer/src/cache/kv_quant.rs:112-154) and attends over f32 pages; this is the form that attention reads directly.
+ * codes [num_pages][n_kv_heads][page_size][head_dim] E4M3; scales [num_pages][n_kv_heads] E8M0 bytes (value = code * 2^(byte - 127)),
+ * page_size 16, 32, 64 or 128, head_dim 64 or 128 (else B2Q_ERR_UNSUPPORTED).  Sequence b: q_starts [seqs + 1] gives its rows
+ * [q_starts[b], q_starts[b + 1]) among `tokens` rows (NULL: one row each, tokens == seqs), seq_lens[b] its cached tokens with the new
+ * ones included, block_tables [seqs][table_width] its pages; the row i of n has position seq_lens[b] - n + i.  All three are read on the
+ * device.  A sequence whose entries cannot be (offsets that run backwards or past `tokens`, fewer cached tokens than rows, more than
+ * table_width pages hold) is left out and records B2Q_ERR_INVALID_DIMENSION; a table entry outside [0, num_pages) records
+ * B2Q_ERR_INVALID_ARGUMENT and counts as a page that is not there (b2q_check reads both).  Rows outside every sequence are left as they
+ * were.  Neither call uses a workspace: calls on several streams and captured graphs are independent of one another. ---- */
+/* Writes k / v (bf16 [tokens][n_kv_heads][head_dim], ld_k / ld_v elements from token to token) into the pages of their positions.  The scale
+ * of a page and head is 2^e, e the smallest integer in [-50, 119] with absmax <= 448 * 2^e over the tokens it holds; it grows with later
+ * tokens (the codes that are there are encoded again) and never shrinks while the page holds older tokens.  A page whose first token is
+ * among the new ones starts afresh.  NaN is stored as 0, an infinity as the largest code; both record B2Q_ERR_NON_FINITE_FP8.
+ * A page that receives tokens must belong to one sequence (shared prefixes: whole pages). */
+int32_t b2q_kv8_append_bf16(b2q_handle h, const void* k, const void* v, int64_t ld_k, int64_t ld_v, int64_t tokens, const int32_t* q_starts,
+                            const int32_t* seq_lens, const int32_t* block_tables, int64_t seqs, int64_t table_width, int64_t num_pages,
+                            int64_t page_size, int64_t n_kv_heads, int64_t head_dim, uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_scales,
+                            uint8_t* v_scales);
+/* out [tokens][n_heads][head_dim] bf16 = softmax(scale * q k^T) v over the keys at positions <= the row's own, with window > 0 the last
+ * `window` of them; query head g reads kv head g / (n_heads / n_kv_heads).  lse (optional, f32 [tokens][n_heads]) receives the natural
+ * logarithm of the softmax denominators.  A row that sees no key gives zeros and -inf.  Scores, maxima, sums and outputs are held in f32; a
+ * query element keeps an absolute error of 2^-17 of its row's largest, a softmax weight a relative one of 2^-9. */
+int32_t b2q_kv8_attention_bf16(b2q_handle h, const void* q, int64_t ld_q, int64_t tokens, int64_t n_heads, const int32_t* q_starts,
+                               const int32_t* seq_lens, const int32_t* block_tables, int64_t seqs, int64_t table_width, int64_t num_pages,
+                               int64_t page_size, int64_t n_kv_heads, int64_t head_dim, const uint8_t* k_codes, const uint8_t* v_codes,
+                               const uint8_t* k_scales, const uint8_t* v_scales, float scale, int64_t window, void* out, float* lse);
+
 /* ---- KvCacheQuantizer: crates/oxicuda-quant/src/scheme/kv_cache.rs ---- */
 typedef enum { B2Q_KV_PER_TOKEN = 0, B2Q_KV_PER_CHANNEL = 1 } b2q_kv_axis;  /* KvAxis, kv_cache.rs:33-38 */
 /* quantize (:146-221): x is [n_tokens x head_dim] row-major; codes (one per byte, as the reference's Vec<u8>) lie in
@@ -304,6 +346,11 @@ typedef struct {
   float alpha, beta; const float* bias; int32_t epilogue; int32_t w_layout;
 } b2q_gemm_fp8_desc;
 int32_t b2q_gemm_fp8_ex(b2q_handle h, const b2q_gemm_fp8_desc* d);
+/* The product of block-128 operands: out[m,n] = sum_b scale_a[m, b] * scale_w[n / 128, b] * sum_{k in block b} A[m,k] * W[n,k], every block of
+ * 128 along K accumulated in f32 and scaled before it is added in f32.  scale_a [M x ceil(K/128)], scale_w [ceil(N/128) x ceil(K/128)].
+ * Validation as b2q_gemm_fp8; any K (row pitches that TMA cannot take, K % 16 != 0 or operands off a 16-byte boundary, run a plain kernel). */
+int32_t b2q_gemm_fp8_block128(b2q_handle h, const uint8_t* a, const uint8_t* w, int64_t M, int64_t N, int64_t K, int fmt,
+                              const float* scale_a, const float* scale_w, void* out, int out_type);
 /* Checker path on the GPU: software decode (reference or IEEE), k-ascending fp32 FMA, one thread per output
  * — the arithmetic of the reference's naive kernel (crates/oxicuda-ptx/src/templates/gemm.rs:373-447). */
 int32_t b2q_gemm_fp8_simt(b2q_handle h, const uint8_t* a, const uint8_t* w, int64_t M, int64_t N, int64_t K, int fmt,

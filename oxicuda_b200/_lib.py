@@ -196,6 +196,12 @@ SIGNATURES = {
     "b2q_mlp_swiglu_fp8_forward_ex": (C.c_int32, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _P]),
     "b2q_interleave_rows128": (C.c_int32, [_H, _P, _P, _I64, _I64, _P]),
     "b2q_gemm_fp4_blockscaled": (C.c_int32, [_H, _P, _P, _P, _I64, _I64, _I64, _I, _P, _I]),
+    "b2q_gemm_fp8_block128": (C.c_int32, [_H, _P, _P, _I64, _I64, _I64, _I, _P, _P, _P, _I]),
+    "b2q_rms_norm_quantize_fp8_block128_bf16": (C.c_int32, [_H, _P, _P, _P, _I64, _I64, _F, _I, _I, _P, _P, _P]),
+    "b2q_swiglu_quantize_fp8_block128_bf16": (C.c_int32, [_H, _P, _P, _I64, _I64, _I64, _I, _I, _P, _P]),
+    "b2q_kv8_append_bf16": (C.c_int32, [_H, _P, _P, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P]),
+    "b2q_kv8_attention_bf16": (C.c_int32, [_H, _P, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _F, _I64, _P,
+                                           _P]),
     "b2q_classify_workload": (C.c_int32, [_U32, _U32, _U32]),
     "b2q_ref_tile_config": (C.c_int32, [_I, _U32, _U32, _U32, C.POINTER(TileConfig)]),
     "b2q_fp8_compute_split_k": (_U32, [_U32, _U32, _U32]),
@@ -303,3 +309,12 @@ def default_handle(device: int | None = None) -> Handle:
         h = _default[device] = Handle(device)
     h.set_stream(torch.cuda.current_stream(device).cuda_stream)
     return h
+
+
+def require_cuda(who: str, **tensors):
+    """The tensors of a call (None entries left out) lie on the current device: kernels launch there."""
+    import torch
+    device = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for name, t in tensors.items():
+        if t is not None and t.get_device() != device:     # -1 for a host tensor
+            raise InvalidArgument(ERR_INVALID_ARGUMENT, f"{who}: {name} must be on the current CUDA device, got {t.device}")

@@ -183,6 +183,34 @@ def gemm_fp8(a: torch.Tensor, w: torch.Tensor, scale_a: torch.Tensor, scale_w: t
     return out
 
 
+def gemm_fp8_block128(a: torch.Tensor, w: torch.Tensor, scale_a: torch.Tensor, scale_w: torch.Tensor, out: torch.Tensor = None,
+                      out_dtype=torch.bfloat16, fmt: int = L.FP8_E4M3) -> torch.Tensor:
+    """out[M,N] = sum over blocks b of 128 along K of scale_a[m,b] * scale_w[n/128,b] * (A[m,b] . W[n,b]): FP8 codes whose scales go
+    per (row, 128 columns) of A [M,K] and per 128 x 128 block of W [N,K], f32 scales, f32 accumulation.  No counterpart in the
+    reference (its FP8 scales go per tensor)."""
+    if a.dim() != 2 or w.dim() != 2 or a.element_size() != 1 or w.element_size() != 1:
+        raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, "gemm_fp8_block128 takes two matrices of 8-bit codes")
+    M, K = a.shape
+    N, K2 = w.shape
+    if K != K2:
+        raise L.DimensionMismatch(L.ERR_DIMENSION_MISMATCH, f"inner dimensions differ: {K} vs {K2}")
+    kb = -(-K // 128)
+    for s, shape in ((scale_a, (M, kb)), (scale_w, (-(-N // 128), kb))):
+        if s.dtype != torch.float32 or tuple(s.shape) != shape:
+            raise L.DimensionMismatch(L.ERR_DIMENSION_MISMATCH, f"expected f32 scales {list(shape)}, got {s.dtype} {list(s.shape)}")
+    if out is None:
+        if out_dtype not in (torch.bfloat16, torch.float32):
+            raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, f"gemm_fp8_block128: out_dtype must be bfloat16 or float32, got {out_dtype}")
+        out = torch.empty(M, N, dtype=out_dtype, device=a.device)
+    elif tuple(out.shape) != (M, N) or out.dtype not in (torch.bfloat16, torch.float32) or not out.is_contiguous():
+        raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, "gemm_fp8_block128: out must be a contiguous bf16 or f32 tensor [M, N]")
+    L.require_cuda("gemm_fp8_block128", a=a, w=w, scale_a=scale_a, scale_w=scale_w, out=out)
+    a, w, scale_a, scale_w = a.contiguous(), w.contiguous(), scale_a.contiguous(), scale_w.contiguous()
+    default_handle().call("b2q_gemm_fp8_block128", ptr(a), ptr(w), M, N, K, fmt, ptr(scale_a), ptr(scale_w), ptr(out),
+                          L.OUT_BF16 if out.dtype == torch.bfloat16 else L.OUT_F32)
+    return out
+
+
 class EpilogueOp(Enum):
     """EpilogueOp, crates/oxicuda-blas/src/level3/gemm/epilogue.rs:29-45."""
     LinearCombination = 0

@@ -1,0 +1,79 @@
+// The paged 8-bit KV cache shared by its append and attention kernels.
+//   codes  E4M3, [num_pages][n_kv_heads][page_size][head_dim]: the tokens of one page and head are one contiguous tile
+//   scales E8M0 bytes, [num_pages][n_kv_heads]: value = code * 2^(byte - 127), one scale for the page_size x head_dim tile
+// A sequence's token at position p lies in page table[p / page_size], slot p % page_size.
+#pragma once
+
+#include "common.cuh"
+
+namespace kv8 {
+
+struct Batch {                      // which rows and which cached tokens belong to which sequence
+  const int32_t* q_starts;          // [seqs + 1] row offsets of the new tokens, or null: sequence b has row b and no other
+  const int32_t* seq_lens;          // [seqs] cached tokens, the new ones included
+  const int32_t* table;             // [seqs][table_width]
+  int seqs, table_width, tokens;
+  int64_t num_pages;
+  int page_shift, n_kv_heads;
+  int32_t* status;
+};
+
+__device__ __forceinline__ void report(int32_t* status, int code) { atomicCAS(status, 0, code); }
+
+struct Rows { int r0, n, len; };    // first row, new tokens, cached tokens
+// The rows of sequence b; an impossible entry (offsets that run backwards or out of the rows, fewer cached tokens than new
+// ones, more than the table holds) counts as no rows, and is reported.
+__device__ __forceinline__ Rows rows_of(const Batch& t, int b, bool tell) {
+  Rows r;
+  r.r0 = t.q_starts ? t.q_starts[b] : b;
+  r.n = t.q_starts ? t.q_starts[b + 1] - r.r0 : 1;
+  r.len = t.seq_lens[b];
+  const bool ok = r.r0 >= 0 && r.n >= 0 && r.n <= t.tokens && r.r0 <= t.tokens - r.n && r.len >= r.n &&
+                  (int64_t)r.len <= ((int64_t)t.table_width << t.page_shift);
+  if (!ok) {
+    if (tell) report(t.status, B2Q_ERR_INVALID_DIMENSION);
+    r.n = 0; r.len = 0;
+  }
+  return r;
+}
+// page of the given index of a sequence, or -1 (reported) when the table names none
+__device__ __forceinline__ int page_of(const Batch& t, int b, int index, bool tell) {
+  const int pg = t.table[(int64_t)b * t.table_width + index];
+  if (pg < 0 || pg >= t.num_pages) {
+    if (tell) report(t.status, B2Q_ERR_INVALID_ARGUMENT);
+    return -1;
+  }
+  return pg;
+}
+
+// Finds the unit'th item of a list in which sequence b has count(b) items, by a whole warp: {b, index within b}, b = -1 past the end.
+template <typename F>
+__device__ __forceinline__ int2 find_unit(int seqs, int64_t unit, F count) {
+  const int lane = threadIdx.x & 31;
+  for (int b0 = 0; b0 < seqs; b0 += 32) {
+    const int c = b0 + lane < seqs ? count(b0 + lane) : 0;
+    int64_t s = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += up;
+    }
+    const int64_t total = __shfl_sync(0xffffffffu, s, 31);
+    if (unit < total) {
+      const unsigned hit = __ballot_sync(0xffffffffu, s > unit);
+      const int src = __ffs(hit) - 1;
+      const int64_t before = __shfl_sync(0xffffffffu, s - c, src);
+      return make_int2(b0 + src, (int)(unit - before));
+    }
+    unit -= total;
+  }
+  return make_int2(-1, 0);
+}
+
+__device__ __forceinline__ float pow2_byte(uint32_t e8m0) { return e8m0_to_f32_dev(e8m0); }
+
+}  // namespace kv8
+
+// The checks of a batch that append and attention share (kv8_append.cu).
+int32_t b2q_kv8_batch(b2q_handle h, const char* who, int64_t tokens, const int32_t* q_starts, const int32_t* seq_lens, const int32_t* block_tables,
+                      int64_t seqs, int64_t table_width, int64_t num_pages, int64_t page_size, int64_t n_kv_heads, int64_t head_dim, kv8::Batch* out);

@@ -1,0 +1,175 @@
+// New keys and values into the paged 8-bit cache (layout: kv8.cuh).
+//
+// The scale of a page and head is 2^e with the smallest e for which absmax <= 448 * 2^e over the tokens the page holds
+// (clamped to [-50, 119]): a power of two costs an E4M3 code no precision but where it falls below the normal range, and
+// lets a page's scale grow later by re-encoding its codes exactly (again but for subnormals).  Page and head belong to
+// one warp: it takes the absmax of the new tokens that fall into the page, raises the page's scale if it must (a page that
+// held tokens before never shrinks its scale), re-encodes the tokens already there, and writes the new ones.  No atomics:
+// the result does not depend on the order in which pages are written.
+// A NaN is stored as 0 and an infinity as the largest code, and B2Q_ERR_NON_FINITE_FP8 is recorded.
+// Bound by latency for single tokens (two dependent reads), else by HBM: 2 bytes read and 1 written per channel.
+#include "kv8.cuh"
+
+namespace kv8 {
+
+constexpr int kMinExp = -50, kMaxExp = 119;
+
+struct AppendArgs {
+  Batch t;
+  const __nv_bfloat16* x[2]; int64_t ld[2];      // keys, values: [tokens][n_kv_heads][head_dim], ld elements from token to token
+  uint8_t* codes[2]; uint8_t* scales[2];
+  int units;                                     // upper bound of (sequence, page) pairs that receive tokens
+};
+
+// smallest e with amax <= 448 * 2^e (448 = 1.75 * 2^8)
+__device__ __forceinline__ int scale_exp(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  return min(kMaxExp, max(kMinExp, e));          // a subnormal or zero amax ends at kMinExp
+}
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // e in [-126, 127]
+
+template <int D>
+__global__ void __launch_bounds__(128) kv8_append_kernel(const AppendArgs p) {
+  constexpr int LPR = D / 8, RPW = 32 / LPR;     // lanes per token row (16-byte loads), rows a warp takes at once
+  b2q_pdl_entry();
+  const Batch& t = p.t;
+  const int lane = threadIdx.x & 31, sub = lane % LPR, row = lane / LPR;
+  const int ps = 1 << t.page_shift;
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int per = 2 * t.n_kv_heads;
+  if (item >= (int64_t)p.units * per) return;
+  const int unit = (int)(item / per), head = (int)(item % per) >> 1, kv = (int)(item & 1);
+  const bool tell = head == 0 && kv == 0;
+  int2 f;
+  if (t.q_starts == nullptr) f = make_int2(unit, 0);
+  else {
+    if (unit == 0 && tell) for (int b = lane; b < t.seqs; b += 32) rows_of(t, b, true);
+    f = find_unit(t.seqs, unit, [&](int b) {
+      const Rows r = rows_of(t, b, false);
+      return r.n > 0 ? ((r.len - 1) >> t.page_shift) - ((r.len - r.n) >> t.page_shift) + 1 : 0;
+    });
+    if (f.x < 0) return;
+  }
+  const Rows r = rows_of(t, f.x, tell && lane == 0 && t.q_starts == nullptr);
+  if (r.n == 0) return;
+  const int first = r.len - r.n;                                        // position of the first new token
+  const int index = (first >> t.page_shift) + f.y;
+  const int pg = page_of(t, f.x, index, tell && lane == 0);
+  if (pg < 0) return;
+  const int base = index << t.page_shift;
+  const int lo = max(first, base), hi = min(r.len, base + ps);          // positions that this page receives
+  const int held = lo - base;                                           // tokens it holds already
+  const __nv_bfloat16* x = p.x[kv] + (int64_t)(r.r0 + lo - first) * p.ld[kv] + (int64_t)head * D;
+  const int64_t tile = ((int64_t)pg * t.n_kv_heads + head);
+  uint8_t* codes = p.codes[kv] + ((tile << t.page_shift)) * D;
+  const int old = held > 0 ? (int)p.scales[kv][tile] - 127 : kMinExp;
+
+  float amax = 0.0f;
+  bool bad = false;
+  for (int i = row; i < hi - lo; i += RPW) {
+    const uint4 q = *reinterpret_cast<const uint4*>(x + (int64_t)i * p.ld[kv] + sub * 8);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const float v = fabsf(__uint_as_float(s ? (w[j] & 0xFFFF0000u) : (w[j] << 16)));
+        const bool fin = v < INFINITY;
+        bad |= !fin;
+        amax = fmaxf(amax, fin ? v : 0.0f);
+      }
+    }
+  }
+  amax = warp_max(amax);
+  if (__any_sync(0xffffffffu, bad) && lane == 0) report(t.status, B2Q_ERR_NON_FINITE_FP8);
+  const int e = max(old, scale_exp(amax));
+  if (held > 0 && e > old) {                                            // the tokens already there move to the larger scale
+    const float f2 = pow2f(max(old - e, -126));
+    for (int i = row; i < held; i += RPW) {
+      uint2* c = reinterpret_cast<uint2*>(codes + (int64_t)i * D + sub * 8);
+      const uint2 was = *c;
+      uint32_t w[2] = {was.x, was.y}, o[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t half[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[j] >> (16 * s)), __NV_E4M3);
+          const float2 v = __half22float2(__half2(hr));
+          half[s] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v.x * f2, v.y * f2), __NV_SATFINITE, __NV_E4M3);
+        }
+        o[j] = half[0] | (half[1] << 16);
+      }
+      *c = make_uint2(o[0], o[1]);
+    }
+  }
+  const float inv = pow2f(-e);
+  for (int i = row; i < hi - lo; i += RPW) {
+    const uint4 q = *reinterpret_cast<const uint4*>(x + (int64_t)i * p.ld[kv] + sub * 8);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float a = __uint_as_float(w[j] << 16) * inv, b = __uint_as_float(w[j] & 0xFFFF0000u) * inv;
+      a = a == a ? a : 0.0f;
+      b = b == b ? b : 0.0f;
+      o[j] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    }
+    *reinterpret_cast<uint2*>(codes + (int64_t)(held + i) * D + sub * 8) = make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
+  }
+  if (lane == 0) p.scales[kv][tile] = (uint8_t)(e + 127);
+}
+
+}  // namespace kv8
+
+extern "C" int32_t b2q_kv8_append_bf16(b2q_handle h, const void* k, const void* v, int64_t ld_k, int64_t ld_v, int64_t tokens, const int32_t* q_starts,
+                                       const int32_t* seq_lens, const int32_t* block_tables, int64_t seqs, int64_t table_width, int64_t num_pages,
+                                       int64_t page_size, int64_t n_kv_heads, int64_t head_dim, uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_scales,
+                                       uint8_t* v_scales) {
+  B2Q_REQUIRE_HANDLE(h);
+  kv8::AppendArgs p{};
+  int32_t st = b2q_kv8_batch(h, "kv8_append", tokens, q_starts, seq_lens, block_tables, seqs, table_width, num_pages, page_size, n_kv_heads, head_dim, &p.t);
+  if (st != B2Q_OK) return st;
+  if (!k || !v || !k_codes || !v_codes || !k_scales || !v_scales) B2Q_FAIL(h, B2Q_ERR_INVALID_ARGUMENT, "kv8_append: null pointer");
+  if (ld_k < n_kv_heads * head_dim || ld_v < n_kv_heads * head_dim || ld_k % 8 != 0 || ld_v % 8 != 0 ||
+      ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_codes) | reinterpret_cast<uintptr_t>(v_codes)) & 15) != 0)
+    B2Q_FAIL(h, B2Q_ERR_INVALID_ARGUMENT, "kv8_append: tensors must be 16-byte aligned, token strides multiples of 8 elements and at least n_kv_heads * head_dim");
+  p.x[0] = static_cast<const __nv_bfloat16*>(k); p.x[1] = static_cast<const __nv_bfloat16*>(v);
+  p.ld[0] = ld_k; p.ld[1] = ld_v;
+  p.codes[0] = k_codes; p.codes[1] = v_codes; p.scales[0] = k_scales; p.scales[1] = v_scales;
+  // a sequence with n new tokens touches at most (n - 1) / page_size + 2 pages, and never more than n
+  int64_t units = tokens;
+  if (q_starts && tokens / page_size + 2 * seqs < units) units = tokens / page_size + 2 * seqs;
+  p.units = (int)units;
+  const int64_t ctas = ceil_div64(units * 2 * n_kv_heads, 4);
+  if (ctas > 0x7FFFFFFF) B2Q_FAIL(h, B2Q_ERR_INVALID_DIMENSION, "kv8_append: %lld tokens are too many", (long long)tokens);
+  B2Q_CUDA(h, b2q_pdl_launch(h->sw.chain_pdl != 0, head_dim == 64 ? kv8::kv8_append_kernel<64> : kv8::kv8_append_kernel<128>, dim3((unsigned)ctas), dim3(128), 0,
+                             h->stream, p));
+  return B2Q_OK;
+}
+
+// The checks of a batch that append and attention share.
+int32_t b2q_kv8_batch(b2q_handle h, const char* who, int64_t tokens, const int32_t* q_starts, const int32_t* seq_lens, const int32_t* block_tables,
+                      int64_t seqs, int64_t table_width, int64_t num_pages, int64_t page_size, int64_t n_kv_heads, int64_t head_dim, kv8::Batch* out) {
+  if (tokens <= 0 || seqs <= 0) B2Q_FAIL(h, B2Q_ERR_EMPTY_INPUT, "%s: empty batch (%lld tokens, %lld sequences)", who, (long long)tokens, (long long)seqs);
+  if (table_width <= 0 || num_pages <= 0 || n_kv_heads <= 0)
+    B2Q_FAIL(h, B2Q_ERR_INVALID_DIMENSION, "%s: dimensions must be non-zero: table_width=%lld, num_pages=%lld, n_kv_heads=%lld", who, (long long)table_width,
+             (long long)num_pages, (long long)n_kv_heads);
+  if (!seq_lens || !block_tables) B2Q_FAIL(h, B2Q_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  if (!q_starts && tokens != seqs)
+    B2Q_FAIL(h, B2Q_ERR_DIMENSION_MISMATCH, "%s: without q_starts every sequence has one token: expected %lld tokens, got %lld", who, (long long)seqs, (long long)tokens);
+  if (head_dim != 64 && head_dim != 128) B2Q_FAIL(h, B2Q_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128, got %lld", who, (long long)head_dim);
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
+    B2Q_FAIL(h, B2Q_ERR_UNSUPPORTED, "%s: page_size must be 16, 32, 64 or 128, got %lld", who, (long long)page_size);
+  if (tokens > (1 << 30) || seqs > (1 << 24) || n_kv_heads > 4096 || table_width > (1 << 24) || (table_width * page_size) > 0x7FFFFFFF ||
+      num_pages > 0x7FFFFFFF / (n_kv_heads * page_size))
+    B2Q_FAIL(h, B2Q_ERR_INVALID_DIMENSION, "%s: too large: tokens=%lld, sequences=%lld, table_width=%lld, num_pages=%lld", who, (long long)tokens,
+             (long long)seqs, (long long)table_width, (long long)num_pages);
+  out->q_starts = q_starts; out->seq_lens = seq_lens; out->table = block_tables;
+  out->seqs = (int)seqs; out->table_width = (int)table_width; out->tokens = (int)tokens;
+  out->num_pages = num_pages; out->page_shift = page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7;
+  out->n_kv_heads = (int)n_kv_heads;
+  out->status = h->d_status;
+  return B2Q_OK;
+}

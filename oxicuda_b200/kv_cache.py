@@ -221,3 +221,117 @@ def rms_norm_quantize_fp8(x: torch.Tensor, gamma: torch.Tensor, eps: float, resi
     default_handle().call("b2q_rms_norm_quantize_fp8_bf16", ptr(x), ptr(residual), ptr(gamma.contiguous()), rows, cols, float(eps), fmt,
                           rounding, ptr(scales), ptr(codes), ptr(y))
     return (codes, scales, y) if want_y else (codes, scales)
+
+
+def rms_norm_quantize_fp8_block128(x: torch.Tensor, gamma: torch.Tensor, eps: float, residual: torch.Tensor = None, fmt: int = L.FP8_E4M3,
+                                   rounding: int = L.ROUND_RNE, want_y: bool = False):
+    """rms_norm_quantize_fp8 with one scale per (row, 128 columns), the operand of blas.gemm_fp8_block128.  `residual` (bf16, x's
+    shape) is updated in place with residual + x and normalised instead of x.  Returns (codes u8 [rows, cols], scales f32
+    [rows, ceil(cols / 128)]) and y (bf16) when asked."""
+    if x.dtype != torch.bfloat16 or gamma.dtype != torch.bfloat16 or x.dim() != 2:
+        raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, "rms_norm_quantize_fp8_block128 takes a bf16 matrix and a bf16 gamma")
+    rows, cols = x.shape
+    if rows == 0 or cols == 0:
+        raise L.EmptyInput(L.ERR_EMPTY_INPUT, "rms_norm_quantize_fp8_block128")
+    if gamma.numel() != cols:
+        raise L.DimensionMismatch(L.ERR_DIMENSION_MISMATCH, f"expected {cols}, got {gamma.numel()}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != torch.bfloat16 or not residual.is_contiguous()):
+        raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, "residual must be a contiguous bf16 tensor of x's shape")
+    L.require_cuda("rms_norm_quantize_fp8_block128", x=x, gamma=gamma, residual=residual)
+    x, gamma = x.contiguous(), gamma.contiguous()
+    codes = torch.empty(rows, cols, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(rows, -(-cols // 128), dtype=torch.float32, device=x.device)
+    y = torch.empty_like(x) if want_y else None
+    default_handle().call("b2q_rms_norm_quantize_fp8_block128_bf16", ptr(x), ptr(residual), ptr(gamma), rows, cols, float(eps), fmt, rounding,
+                          ptr(scales), ptr(codes), ptr(y))
+    return (codes, scales, y) if want_y else (codes, scales)
+
+
+class PagedFp8KvCache:
+    """A paged KV cache in E4M3 codes with one power-of-two scale (an E8M0 byte) per page and kv head, and the attention that reads
+    it.  Codes u8 [num_pages, n_kv_heads, page_size, head_dim], scales u8 [num_pages, n_kv_heads]; head_dim 64 or 128, page_size 16,
+    32, 64 or 128.  The tensors belong to the caller, who may share them with other code."""
+
+    PAGE_SIZES = (16, 32, 64, 128)
+    HEAD_DIMS = (64, 128)
+
+    def __init__(self, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor):
+        if k_codes.dim() != 4:
+            raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, "PagedFp8KvCache: codes must be [num_pages, n_kv_heads, page_size, head_dim]")
+        self.num_pages, self.n_kv_heads, self.page_size, self.head_dim = k_codes.shape
+        if self.page_size not in self.PAGE_SIZES or self.head_dim not in self.HEAD_DIMS:
+            raise L.UnsupportedOperation(L.ERR_UNSUPPORTED, f"PagedFp8KvCache: page_size must be one of {list(self.PAGE_SIZES)} and head_dim one of "
+                                         f"{list(self.HEAD_DIMS)}, got {self.page_size} and {self.head_dim}")
+        for t, shape in ((k_codes, k_codes.shape), (v_codes, k_codes.shape), (k_scales, k_codes.shape[:2]), (v_scales, k_codes.shape[:2])):
+            if t.dtype != torch.uint8 or t.shape != shape or not t.is_contiguous():
+                raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, f"PagedFp8KvCache: expected a contiguous uint8 tensor {list(shape)}, got {t.dtype} {list(t.shape)}")
+        self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
+
+    @staticmethod
+    def empty(num_pages: int, page_size: int, n_kv_heads: int, head_dim: int, device) -> "PagedFp8KvCache":
+        codes = [torch.zeros(num_pages, n_kv_heads, page_size, head_dim, dtype=torch.uint8, device=device) for _ in range(2)]
+        scales = [torch.full((num_pages, n_kv_heads), 127, dtype=torch.uint8, device=device) for _ in range(2)]
+        return PagedFp8KvCache(*codes, *scales)
+
+    def _rows(self, who: str, x: torch.Tensor, heads: int):
+        """x as [tokens, heads, head_dim] whose heads are packed: a view of a wider GEMM result is taken as it is."""
+        if x.dtype != torch.bfloat16 or x.dim() != 3 or x.shape[2] != self.head_dim or (heads and x.shape[1] != heads):
+            raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, f"{who}: expected bf16 [tokens, {heads or 'heads'}, {self.head_dim}], got {x.dtype} {list(x.shape)}")
+        width = x.shape[1] * self.head_dim
+        ld = x.stride(0) if x.shape[0] > 1 else width
+        if x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != self.head_dim) or ld < width or ld % 8 or x.data_ptr() % 16:
+            x = x.clone(memory_format=torch.contiguous_format)
+            ld = width
+        return x, ld
+
+    def _batch(self, who: str, tokens: int, seq_lens: torch.Tensor, block_tables: torch.Tensor, q_starts):
+        if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or block_tables.dtype != torch.int32 or block_tables.dim() != 2:
+            raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, f"{who}: seq_lens [seqs] and block_tables [seqs, width] are int32 tensors")
+        seqs = seq_lens.numel()
+        if tokens == 0 or seqs == 0:
+            raise L.EmptyInput(L.ERR_EMPTY_INPUT, f"{who}: empty batch")
+        if block_tables.shape[0] != seqs:
+            raise L.DimensionMismatch(L.ERR_DIMENSION_MISMATCH, f"expected {seqs} block tables, got {block_tables.shape[0]}")
+        if q_starts is None and tokens != seqs:
+            raise L.DimensionMismatch(L.ERR_DIMENSION_MISMATCH, f"expected {seqs} tokens (one per sequence without q_starts), got {tokens}")
+        if q_starts is not None and (q_starts.dtype != torch.int32 or q_starts.dim() != 1 or q_starts.numel() != seqs + 1):
+            raise L.DimensionMismatch(L.ERR_DIMENSION_MISMATCH, f"expected int32 q_starts [{seqs + 1}], got {q_starts.dtype} {list(q_starts.shape)}")
+        return seq_lens.contiguous(), block_tables.contiguous(), None if q_starts is None else q_starts.contiguous(), seqs
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, seq_lens: torch.Tensor, block_tables: torch.Tensor, q_starts: torch.Tensor = None) -> None:
+        """Writes new keys and values (bf16 [tokens, n_kv_heads, head_dim]) into their pages.  seq_lens int32 [seqs]: cached tokens with
+        the new ones included; block_tables int32 [seqs, width]; q_starts int32 [seqs + 1]: row offsets, None for one row per sequence.
+        All on the device and read there: what is wrong with them is recorded, and raised by the handle's check()."""
+        k, ld_k = self._rows("append", k, self.n_kv_heads)
+        v, ld_v = self._rows("append", v, self.n_kv_heads)
+        if k.shape[0] != v.shape[0]:
+            raise L.DimensionMismatch(L.ERR_DIMENSION_MISMATCH, f"expected {k.shape[0]} rows of v, got {v.shape[0]}")
+        seq_lens, block_tables, q_starts, seqs = self._batch("append", k.shape[0], seq_lens, block_tables, q_starts)
+        L.require_cuda("append", k=k, v=v, seq_lens=seq_lens, block_tables=block_tables, q_starts=q_starts, k_codes=self.k_codes, v_codes=self.v_codes,
+                       k_scales=self.k_scales, v_scales=self.v_scales)
+        default_handle().call("b2q_kv8_append_bf16", ptr(k), ptr(v), ld_k, ld_v, k.shape[0], ptr(q_starts), ptr(seq_lens), ptr(block_tables), seqs,
+                              block_tables.shape[1], self.num_pages, self.page_size, self.n_kv_heads, self.head_dim, ptr(self.k_codes),
+                              ptr(self.v_codes), ptr(self.k_scales), ptr(self.v_scales))
+
+    def attend(self, q: torch.Tensor, seq_lens: torch.Tensor, block_tables: torch.Tensor, q_starts: torch.Tensor = None, scale: float = None,
+               window: int = 0, out: torch.Tensor = None, want_lse: bool = False):
+        """Causal attention of q (bf16 [tokens, heads, head_dim], heads a multiple of n_kv_heads) over the cached tokens, the rows' own
+        included; with window > 0 over the last `window` of them.  scale: 1 / sqrt(head_dim) unless given.  Returns out (bf16, q's shape)
+        and, when asked, the log-sum-exp of the scores (f32 [tokens, heads]).  Rows outside every sequence are left as they were (`out`
+        given) or unspecified."""
+        q, ld_q = self._rows("attend", q, 0)
+        tokens, heads, d = q.shape
+        if heads == 0 or heads % self.n_kv_heads != 0:
+            raise L.InvalidDimension(L.ERR_INVALID_DIMENSION, f"{heads} query heads are not a multiple of {self.n_kv_heads} kv heads")
+        seq_lens, block_tables, q_starts, seqs = self._batch("attend", tokens, seq_lens, block_tables, q_starts)
+        if out is None:
+            out = torch.empty(tokens, heads, d, dtype=torch.bfloat16, device=q.device)
+        elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+            raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, "attend: out must be a contiguous bf16 tensor of q's shape")
+        lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if want_lse else None
+        L.require_cuda("attend", q=q, seq_lens=seq_lens, block_tables=block_tables, q_starts=q_starts, out=out, k_codes=self.k_codes,
+                       v_codes=self.v_codes, k_scales=self.k_scales, v_scales=self.v_scales)
+        default_handle().call("b2q_kv8_attention_bf16", ptr(q), ld_q, tokens, heads, ptr(q_starts), ptr(seq_lens), ptr(block_tables), seqs,
+                              block_tables.shape[1], self.num_pages, self.page_size, self.n_kv_heads, d, ptr(self.k_codes), ptr(self.v_codes),
+                              ptr(self.k_scales), ptr(self.v_scales), d ** -0.5 if scale is None else float(scale), int(window), ptr(out), ptr(lse))
+        return (out, lse) if want_lse else out

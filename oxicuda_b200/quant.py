@@ -348,3 +348,42 @@ def int8_dequant(q: torch.Tensor, scale: float) -> torch.Tensor:
     out = torch.empty(qd.numel(), dtype=torch.float32, device=qd.device)
     default_handle().call("b2q_int8_dequant_f32", ptr(qd), qd.numel(), C.c_float(scale), ptr(out))
     return _back(out, was_host)
+
+
+# ---- FP8 with a scale for each block of 128 (the operands of blas.gemm_fp8_block128) ----
+def swiglu_quantize_fp8_block128(gate: torch.Tensor, up: torch.Tensor, fmt: int = L.FP8_E4M3, rounding: int = L.ROUND_RNE):
+    """silu(gate) * up (SwiGluExpert::forward, crates/oxicuda-moe/src/expert/ffn.rs:208-243) in f32, then FP8 codes with one scale per
+    (row, 128 columns), in one kernel.  gate, up: bf16 [rows, cols] on the device, e.g. the two halves of one [rows, 2 * cols] GEMM
+    result.  Returns (codes u8 [rows, cols], scales f32 [rows, ceil(cols / 128)])."""
+    if gate.dtype != torch.bfloat16 or up.dtype != torch.bfloat16 or gate.dim() != 2 or gate.shape != up.shape:
+        raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, "swiglu_quantize_fp8_block128 takes two bf16 matrices of one shape")
+    rows, cols = gate.shape
+    if rows == 0 or cols == 0:
+        raise L.EmptyInput(L.ERR_EMPTY_INPUT, "swiglu_quantize_fp8_block128")
+    L.require_cuda("swiglu_quantize_fp8_block128", gate=gate, up=up)
+    ld = gate.stride(0) if rows > 1 else max(cols, gate.stride(0))
+    if cols > 1 and (gate.stride(1) != 1 or up.stride(1) != 1) or ld < cols or (rows > 1 and up.stride(0) != ld):
+        gate, up, ld = gate.contiguous(), up.contiguous(), cols
+    codes = torch.empty(rows, cols, dtype=torch.uint8, device=gate.device)
+    scales = torch.empty(rows, -(-cols // 128), dtype=torch.float32, device=gate.device)
+    default_handle().call("b2q_swiglu_quantize_fp8_block128_bf16", ptr(gate), ptr(up), rows, cols, ld, fmt, rounding, ptr(scales), ptr(codes))
+    return codes, scales
+
+
+def quantize_fp8_blocks(x: torch.Tensor, block_rows: int, fmt: int = L.FP8_E4M3, rounding: str = "rne"):
+    """FP8 codes of a matrix [rows, cols] with one scale per block of `block_rows` x 128 (1: activations, 128: weights): the rule of
+    Fp8Codec.quantize_rows over each block, on the device.  Returns (codes u8 [rows, cols], scales f32 [ceil(rows / block_rows),
+    ceil(cols / 128)])."""
+    if x.dim() != 2 or block_rows not in (1, 128):
+        raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, "quantize_fp8_blocks takes a matrix and blocks of 1 or 128 rows")
+    rows, cols = x.shape
+    if rows == 0 or cols == 0:
+        raise L.EmptyInput(L.ERR_EMPTY_INPUT, "quantize_fp8_blocks")
+    L.require_cuda("quantize_fp8_blocks", x=x)
+    rb, cb = -(-rows // block_rows), -(-cols // 128)
+    if rb * block_rows != rows or cb * 128 != cols:
+        x = torch.nn.functional.pad(x, (0, cb * 128 - cols, 0, rb * block_rows - rows))
+    blocks = x.view(rb, block_rows, cb, 128).transpose(1, 2).contiguous()
+    codes, scales = (Fp8Codec.e4m3(rounding) if fmt == L.FP8_E4M3 else Fp8Codec.e5m2(rounding)).quantize_rows(blocks, rb * cb, block_rows * 128)
+    codes = codes.view(rb, cb, block_rows, 128).transpose(1, 2).reshape(rb * block_rows, cb * 128)
+    return codes[:rows, :cols].contiguous(), scales.view(rb, cb)

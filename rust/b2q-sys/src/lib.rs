@@ -94,6 +94,10 @@ extern "C" {
     pub fn b2q_distfp8_quantize_block_f32(h: b2q_handle, x: *const f32, n: i64, block: i64, q: *mut u8, absmaxs: *mut f32) -> i32;
     pub fn b2q_distfp8_dequantize_block_f32(h: b2q_handle, q: *const u8, n: i64, block: i64, absmaxs: *const f32, out: *mut f32) -> i32;
     pub fn b2q_rms_norm_quantize_fp8_bf16(h: b2q_handle, x_bf16: *const c_void, residual_bf16: *mut c_void, gamma_bf16: *const c_void, rows: i64, cols: i64, eps: f32, fmt: c_int, rounding: c_int, scales: *mut f32, codes: *mut u8, y_out_bf16: *mut c_void) -> i32;
+    pub fn b2q_rms_norm_quantize_fp8_block128_bf16(h: b2q_handle, x_bf16: *const c_void, residual_bf16: *mut c_void, gamma_bf16: *const c_void, rows: i64, cols: i64, eps: f32, fmt: c_int, rounding: c_int, scales: *mut f32, codes: *mut u8, y_out_bf16: *mut c_void) -> i32;
+    pub fn b2q_swiglu_quantize_fp8_block128_bf16(h: b2q_handle, gate: *const c_void, up: *const c_void, rows: i64, cols: i64, ld: i64, fmt: c_int, rounding: c_int, scales: *mut f32, codes: *mut u8) -> i32;
+    pub fn b2q_kv8_append_bf16(h: b2q_handle, k: *const c_void, v: *const c_void, ld_k: i64, ld_v: i64, tokens: i64, q_starts: *const i32, seq_lens: *const i32, block_tables: *const i32, seqs: i64, table_width: i64, num_pages: i64, page_size: i64, n_kv_heads: i64, head_dim: i64, k_codes: *mut u8, v_codes: *mut u8, k_scales: *mut u8, v_scales: *mut u8) -> i32;
+    pub fn b2q_kv8_attention_bf16(h: b2q_handle, q: *const c_void, ld_q: i64, tokens: i64, n_heads: i64, q_starts: *const i32, seq_lens: *const i32, block_tables: *const i32, seqs: i64, table_width: i64, num_pages: i64, page_size: i64, n_kv_heads: i64, head_dim: i64, k_codes: *const u8, v_codes: *const u8, k_scales: *const u8, v_scales: *const u8, scale: f32, window: i64, out: *mut c_void, lse: *mut f32) -> i32;
     pub fn b2q_kv_cache_quantize_f32(h: b2q_handle, x: *const f32, n_tokens: i64, head_dim: i64, bits: c_int, axis: c_int, codes: *mut u8, scales: *mut f32, zero_points: *mut f32) -> i32;
     pub fn b2q_kv_cache_quantize_bf16(h: b2q_handle, x_bf16: *const c_void, n_tokens: i64, head_dim: i64, bits: c_int, axis: c_int, codes: *mut u8, scales: *mut f32, zero_points: *mut f32) -> i32;
     pub fn b2q_kv_cache_dequantize_f32(h: b2q_handle, codes: *const u8, n_tokens: i64, head_dim: i64, axis: c_int, scales: *const f32, zero_points: *const f32, out: *mut f32) -> i32;
@@ -118,6 +122,7 @@ extern "C" {
     pub fn b2q_gemm_i8(h: b2q_handle, a: *const i8, b: *const i8, M: i64, N: i64, K: i64, c_s32: *mut i32, c_f32: *mut f32, scale_a: *const f32, scale_b: *const f32) -> i32;
     pub fn b2q_gemm_fp8(h: b2q_handle, a: *const u8, w: *const u8, M: i64, N: i64, K: i64, fmt: c_int, scale_a: *const f32, scale_a_kind: c_int, scale_w: *const f32, scale_w_kind: c_int, out: *mut c_void, out_type: c_int) -> i32;
     pub fn b2q_gemm_fp8_ex(h: b2q_handle, d: *const b2q_gemm_fp8_desc) -> i32;
+    pub fn b2q_gemm_fp8_block128(h: b2q_handle, a: *const u8, w: *const u8, M: i64, N: i64, K: i64, fmt: c_int, scale_a: *const f32, scale_w: *const f32, out: *mut c_void, out_type: c_int) -> i32;
     pub fn b2q_gemm_fp8_simt(h: b2q_handle, a: *const u8, w: *const u8, M: i64, N: i64, K: i64, fmt: c_int, decode_mode: c_int, scale_a: *const f32, scale_a_kind: c_int, scale_w: *const f32, scale_w_kind: c_int, out: *mut c_void, out_type: c_int) -> i32;
     pub fn b2q_tp_unique_id(id128: *mut u8) -> i32;
     pub fn b2q_tp_comm_init(id128: *const u8, tp: c_int, rank: c_int, nccl_comm: *mut *mut c_void) -> i32;
