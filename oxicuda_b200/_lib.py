@@ -237,11 +237,17 @@ def ptr(t) -> C.c_void_p:
     return C.c_void_p(t.ctypes.data)
 
 
+def address(t):
+    """Device address of a torch tensor as an int, None (a null pointer) for None."""
+    return None if t is None else t.data_ptr()
+
+
 class Handle:
     """BlasHandle equivalent (crates/oxicuda-blas/src/handle.rs:43-264): one per host thread."""
 
     def __init__(self, device: int = 0):
         self._h = _H()
+        self._stream = 0          # the stream the handle launches on (a new handle: the legacy default stream)
         st = lib().b2q_create(C.byref(self._h), device)
         if st != OK:
             raise _ERRORS.get(st, B2qError)(st, "b2q_create failed (no CUDA device, or not an sm_100 GPU)")
@@ -259,13 +265,14 @@ class Handle:
             pass
 
     def call(self, name: str, *args):
-        st = getattr(lib(), name)(self._h, *args)
+        st = getattr(_lib or lib(), name)(self._h, *args)
         if st != OK:
             msg = lib().b2q_last_error(self._h)
             raise _ERRORS.get(st, B2qError)(st, msg.decode() if msg else name)
 
     def set_stream(self, stream_ptr: int):
         self.call("b2q_set_stream", C.c_void_p(stream_ptr))
+        self._stream = stream_ptr
 
     def set_static_weights(self, static_weights: bool):
         """False: weight operands may be produced by the kernel right before a call (see include/b2q.h)."""
@@ -307,14 +314,20 @@ def default_handle(device: int | None = None) -> Handle:
     h = _default.get(device)
     if h is None:
         h = _default[device] = Handle(device)
-    h.set_stream(torch.cuda.current_stream(device).cuda_stream)
+    stream = torch._C._cuda_getCurrentRawStream(device)    # what torch.cuda.current_stream(device).cuda_stream is
+    if stream != h._stream:
+        h.set_stream(stream)
     return h
 
 
 def require_cuda(who: str, **tensors):
     """The tensors of a call (None entries left out) lie on the current device: kernels launch there."""
     import torch
-    device = torch.cuda.current_device() if torch.cuda.is_available() else None
+    device = None
     for name, t in tensors.items():
-        if t is not None and t.get_device() != device:     # -1 for a host tensor
-            raise InvalidArgument(ERR_INVALID_ARGUMENT, f"{who}: {name} must be on the current CUDA device, got {t.device}")
+        if t is not None:
+            on = t.get_device()                            # -1 for a host tensor
+            if device is None:
+                device = torch.cuda.current_device() if on >= 0 else None
+            if on < 0 or on != device:
+                raise InvalidArgument(ERR_INVALID_ARGUMENT, f"{who}: {name} must be on the current CUDA device, got {t.device}")

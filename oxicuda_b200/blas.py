@@ -206,7 +206,7 @@ def gemm_fp8_block128(a: torch.Tensor, w: torch.Tensor, scale_a: torch.Tensor, s
         raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, "gemm_fp8_block128: out must be a contiguous bf16 or f32 tensor [M, N]")
     L.require_cuda("gemm_fp8_block128", a=a, w=w, scale_a=scale_a, scale_w=scale_w, out=out)
     a, w, scale_a, scale_w = a.contiguous(), w.contiguous(), scale_a.contiguous(), scale_w.contiguous()
-    default_handle().call("b2q_gemm_fp8_block128", ptr(a), ptr(w), M, N, K, fmt, ptr(scale_a), ptr(scale_w), ptr(out),
+    default_handle().call("b2q_gemm_fp8_block128", a.data_ptr(), w.data_ptr(), M, N, K, fmt, scale_a.data_ptr(), scale_w.data_ptr(), out.data_ptr(),
                           L.OUT_BF16 if out.dtype == torch.bfloat16 else L.OUT_F32)
     return out
 

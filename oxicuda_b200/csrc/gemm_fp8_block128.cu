@@ -95,7 +95,6 @@ __device__ __forceinline__ void umma_pair(uint32_t tmem_d, uint64_t adesc, uint6
       ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
-__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t x, uint64_t y) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(x), "l"(y)); }
 __device__ __forceinline__ float lo32(uint64_t v) { return __uint_as_float((uint32_t)v); }
 __device__ __forceinline__ float hi32(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 
@@ -403,6 +402,9 @@ int32_t launch_pair(b2q_handle h, const uint8_t* a, const uint8_t* w, Params p, 
 
 }  // namespace b128
 
+int32_t b2q_gemm_fp8_block128_few(b2q_handle h, const uint8_t* a, const uint8_t* w, int64_t M, int64_t N, int64_t K, int fmt, const float* scale_a,
+                                  const float* scale_w, void* out, int out_type);
+
 extern "C" int32_t b2q_gemm_fp8_block128(b2q_handle h, const uint8_t* a, const uint8_t* w, int64_t M, int64_t N, int64_t K, int fmt,
                                          const float* scale_a, const float* scale_w, void* out, int out_type) {
   B2Q_REQUIRE_HANDLE(h);
@@ -424,6 +426,7 @@ extern "C" int32_t b2q_gemm_fp8_block128(b2q_handle h, const uint8_t* a, const u
     p.sa = scale_a; p.sw = scale_w; p.out = out;
     p.vec = kb % 4 == 0 && ((reinterpret_cast<uintptr_t>(scale_a) | reinterpret_cast<uintptr_t>(scale_w)) & 15) == 0;
     p.out_type = out_type; p.status = h->d_status;
+    if (M <= 128) return b2q_gemm_fp8_block128_few(h, a, w, M, N, K, fmt, scale_a, scale_w, out, out_type);
     // the tile width whose last wave over the CTA pairs leaves less idle (a 128-wide tile costs a little over half a 256-wide one)
     const int64_t pairs = h->sm_count / 2, tiles128 = ceil_div64(M, 256) * ceil_div64(N, 128);
     const bool wide = ceil_div64(tiles256, pairs) * 100 <= ceil_div64(tiles128, pairs) * 55;

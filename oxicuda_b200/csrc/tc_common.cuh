@@ -136,6 +136,9 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
                ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 
+// two f32 multiply-adds in one instruction: acc = x * y + acc, low and high half
+__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t x, uint64_t y) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(x), "l"(y)); }
+
 // Shared-memory matrix descriptor for a K-major tile stored as rows of 128 bytes with the 128-byte swizzle (what
 // TMA SWIZZLE_128B writes): 8-row groups are 1024 bytes apart (stride byte offset), descriptor version 1, layout
 // type 2.  Advancing K inside the swizzle atom adds the byte offset >> 4 to the start-address field.

@@ -242,8 +242,8 @@ def rms_norm_quantize_fp8_block128(x: torch.Tensor, gamma: torch.Tensor, eps: fl
     codes = torch.empty(rows, cols, dtype=torch.uint8, device=x.device)
     scales = torch.empty(rows, -(-cols // 128), dtype=torch.float32, device=x.device)
     y = torch.empty_like(x) if want_y else None
-    default_handle().call("b2q_rms_norm_quantize_fp8_block128_bf16", ptr(x), ptr(residual), ptr(gamma), rows, cols, float(eps), fmt, rounding,
-                          ptr(scales), ptr(codes), ptr(y))
+    default_handle().call("b2q_rms_norm_quantize_fp8_block128_bf16", x.data_ptr(), L.address(residual), gamma.data_ptr(), rows, cols, float(eps), fmt, rounding,
+                          scales.data_ptr(), codes.data_ptr(), L.address(y))
     return (codes, scales, y) if want_y else (codes, scales)
 
 
@@ -309,9 +309,9 @@ class PagedFp8KvCache:
         seq_lens, block_tables, q_starts, seqs = self._batch("append", k.shape[0], seq_lens, block_tables, q_starts)
         L.require_cuda("append", k=k, v=v, seq_lens=seq_lens, block_tables=block_tables, q_starts=q_starts, k_codes=self.k_codes, v_codes=self.v_codes,
                        k_scales=self.k_scales, v_scales=self.v_scales)
-        default_handle().call("b2q_kv8_append_bf16", ptr(k), ptr(v), ld_k, ld_v, k.shape[0], ptr(q_starts), ptr(seq_lens), ptr(block_tables), seqs,
-                              block_tables.shape[1], self.num_pages, self.page_size, self.n_kv_heads, self.head_dim, ptr(self.k_codes),
-                              ptr(self.v_codes), ptr(self.k_scales), ptr(self.v_scales))
+        default_handle().call("b2q_kv8_append_bf16", k.data_ptr(), v.data_ptr(), ld_k, ld_v, k.shape[0], L.address(q_starts), seq_lens.data_ptr(), block_tables.data_ptr(), seqs,
+                              block_tables.shape[1], self.num_pages, self.page_size, self.n_kv_heads, self.head_dim, self.k_codes.data_ptr(),
+                              self.v_codes.data_ptr(), self.k_scales.data_ptr(), self.v_scales.data_ptr())
 
     def attend(self, q: torch.Tensor, seq_lens: torch.Tensor, block_tables: torch.Tensor, q_starts: torch.Tensor = None, scale: float = None,
                window: int = 0, out: torch.Tensor = None, want_lse: bool = False):
@@ -331,7 +331,7 @@ class PagedFp8KvCache:
         lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if want_lse else None
         L.require_cuda("attend", q=q, seq_lens=seq_lens, block_tables=block_tables, q_starts=q_starts, out=out, k_codes=self.k_codes,
                        v_codes=self.v_codes, k_scales=self.k_scales, v_scales=self.v_scales)
-        default_handle().call("b2q_kv8_attention_bf16", ptr(q), ld_q, tokens, heads, ptr(q_starts), ptr(seq_lens), ptr(block_tables), seqs,
-                              block_tables.shape[1], self.num_pages, self.page_size, self.n_kv_heads, d, ptr(self.k_codes), ptr(self.v_codes),
-                              ptr(self.k_scales), ptr(self.v_scales), d ** -0.5 if scale is None else float(scale), int(window), ptr(out), ptr(lse))
+        default_handle().call("b2q_kv8_attention_bf16", q.data_ptr(), ld_q, tokens, heads, L.address(q_starts), seq_lens.data_ptr(), block_tables.data_ptr(), seqs,
+                              block_tables.shape[1], self.num_pages, self.page_size, self.n_kv_heads, d, self.k_codes.data_ptr(), self.v_codes.data_ptr(),
+                              self.k_scales.data_ptr(), self.v_scales.data_ptr(), d ** -0.5 if scale is None else float(scale), int(window), out.data_ptr(), L.address(lse))
         return (out, lse) if want_lse else out

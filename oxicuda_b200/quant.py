@@ -366,7 +366,7 @@ def swiglu_quantize_fp8_block128(gate: torch.Tensor, up: torch.Tensor, fmt: int 
         gate, up, ld = gate.contiguous(), up.contiguous(), cols
     codes = torch.empty(rows, cols, dtype=torch.uint8, device=gate.device)
     scales = torch.empty(rows, -(-cols // 128), dtype=torch.float32, device=gate.device)
-    default_handle().call("b2q_swiglu_quantize_fp8_block128_bf16", ptr(gate), ptr(up), rows, cols, ld, fmt, rounding, ptr(scales), ptr(codes))
+    default_handle().call("b2q_swiglu_quantize_fp8_block128_bf16", gate.data_ptr(), up.data_ptr(), rows, cols, ld, fmt, rounding, scales.data_ptr(), codes.data_ptr())
     return codes, scales
 
 
