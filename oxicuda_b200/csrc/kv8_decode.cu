@@ -2,30 +2,47 @@
 //   o_i = sum_j softmax_j(scale * q_i . k_j) v_j,  keys j <= pos_i (pos_i = len - n + i), with a window also j > pos_i - window.
 // Bound by HBM: the codes of the visible keys and values are read once; everything else is small.
 //
-// A row is one (new token, query head) pair; the rows of one sequence and kv head that share keys are taken 8 at a time.  The
-// codes feed mma.sync.m16n8k32 (E4M3 x E4M3, f32 sums) as they are stored:
-//   scores   A = the 8 query rows twice: rows 0..7 the E4M3 rounding of q / 2^e, rows 8..15 the E4M3 rounding of what that
-//            leaves, 2^e the power of two that brings the row's largest element into (224, 448].  A bf16 has 8 significant
-//            bits and an E4M3 code 4, so the two terms add up to q exactly but for elements below 2^-9 of the row's largest
-//            (absolute error at most 2^-10 * 2^e, 2^-17 of that element).  B = K as loaded, 4 channels per register.
-//   outputs  A = the weights p = exp2(s - m) * 2^8, split the same way (relative error 2^-9 where a bf16 weight would have
-//            2^-9 too); B = V, whose 4 x 4 byte tiles are transposed in registers (two byte permutations per register).
-// One warp takes 32 keys at a time with its own running maximum and sum, so the main loop has no barrier; warps and the CTAs
-// of a cluster (keys dealt round in tiles of 32) are joined once at the end, through shared and distributed shared memory:
-// no workspace, one launch, and a result that does not depend on timing.
-// The value scale is a power of two 2^lv per page: weights enter as p * 2^(8 + lv - R) and the outputs are kept in units of
-// 2^(R - 8), R following the pages' scales, so the split keeps its precision whatever the pages' sizes are; pages of one tile
-// whose scales lie more than 2^4 apart are multiplied one after the other.
-// Keys behind the last visible one are never read (their codes count as zeros), so stale pages cannot reach a result.
+// A row is one (new token, query head) pair; the rows of one sequence and kv head that share keys are taken 8 * RB at a time.
+// Both products run on mma.sync.m16n8k16 (f16 x f16, f32 sums) with the cache as the 16-row operand and the query rows as the 8
+// columns, so that none of the tensor work is padding for groups of up to 8 heads and an output takes D / 4 registers:
+//   scores^T  [16 keys x 8 rows] = K [16 x D] . Q^T;      outputs^T [16 channels x 8 rows] = V^T [16 x keys] . P^T.
+// An E4M3 code is exact in f16 (one conversion instruction for two).  Q enters as f16 after a power of two has brought its row's
+// largest element into [2^14, 2^15): a bf16 has 8 significant bits and f16 has 11, so it is exact but for elements below 2^-28 of that
+// largest.  The weights enter as p * 2^15 rounded to f16: off by 2^-12 of themselves, or of 2^-29 below the normal range.
+// Channels are dealt to lanes so that a lane's operands are 16 neighbouring bytes of a row (both products sum over, or are independent
+// of, the order of channels); 8 x 8 tiles of P are transposed between lanes by movmatrix, pairs of keys of V by byte permutations.
+// One warp brings tiles of 64 keys into a ring of shared memory by TMA (it alone walks the block table, a batch of tiles ahead); three
+// pairs of warps take the tiles in turn, 32 keys to a warp, each with its own running maximum and sum, so the main loop has no
+// barrier between them.  Warps and the CTAs of a
+// cluster (tiles dealt round) are joined once at the end, through shared and distributed shared memory: no workspace, one
+// launch, and a result that does not depend on timing.
+// The value scale is a power of two 2^lv per page: weights enter as p * 2^(15 + lv - R) and the outputs are kept in units of
+// 2^(R - 15), R following the pages' scales, so the weights keep their precision whatever the pages' sizes are; pages of one tile
+// whose scales lie more than 2^8 apart are multiplied one after the other.
+// Keys behind the last visible one are masked and their value rows zeroed before they are multiplied, so stale codes cannot reach a
+// result; a page that the table does not name is neither read nor counted.
+// Every mbarrier wait is bounded; on expiry the kernel records B2Q_ERR_TIMEOUT and leaves.
 #include "kv8.cuh"
+#include "tc_common.cuh"
 #include <cooperative_groups.h>
 
 namespace cg = cooperative_groups;
 
 namespace kv8 {
 
-constexpr int kWarps = 4, kRows = 8, kTile = 32;
+using namespace tcx;
+
+constexpr int kWarps = 6, kTile = 64;            // consumer warps (pairs); keys of one tile
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr uint64_t kWaitLimitNs = 500000000ull;
+template <int D> struct Ring {
+  static constexpr int kHalf = kTile * D, kStage = 2 * kHalf;          // keys, then values
+  static constexpr int kStages = D == 128 ? 6 : 9;                     // 96 KiB / 72 KiB, two CTAs to an SM
+  static_assert(kStages % (kWarps / 2) == 0, "a stage belongs to one pair of warps, which cannot run a phase ahead of its own");
+  static constexpr int kSmem = kStages * kStage + kStages * 32 + 1024;
+};
 constexpr int kNone = -1000;                     // R of a warp that has seen no page
+constexpr int kSpan = 8;                         // value scales that share a product differ by at most 2^kSpan
 
 struct AttendArgs {
   Batch t;
@@ -37,40 +54,80 @@ struct AttendArgs {
   __nv_bfloat16* out; float* lse;                // [tokens][heads][head_dim], [tokens][heads]
 };
 
-__device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// two values -> two E4M3 codes (low half) and the codes of what the first rounding left
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __nv_fp8x2_storage_t h = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
-  const float2 b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(h, __NV_E4M3)));
-  hi = h;
-  lo = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x - b.x, y - b.y), __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+// four E4M3 codes -> two registers of two f16 (codes 0 and 1, codes 2 and 3)
+__device__ __forceinline__ void to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// over the 8 lanes that share lane & 3
+__device__ __forceinline__ float column_max(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float column_sum(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(min(127, max(-126, e)) + 127) << 23); }
-__device__ __forceinline__ uint4 ld_stream(const uint8_t* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// byte offset of 16-byte unit u of row r in a tile of D-byte rows whose 128-byte lines TMA has swizzled
+template <int D> __device__ __forceinline__ uint32_t swz(int r, int u) {
+  const uint32_t at = (uint32_t)(r * D + u * 16);
+  return at ^ (((at >> 7) & 7) << 4);
+}
+// The key (within its group of 8) that row lr of an operand stands for: an order in which the 16-byte reads of both products meet no
+// bank twice (keys 2 i, 2 i + 1 of the order lie in different halves of the swizzled lines, keys 2 i + e over i in different units).
+template <int D> __device__ __forceinline__ int key_of(int lr) { return (D == 128 ? 0x37156240u : 0x65742130u) >> (4 * lr) & 7; }
 
-template <int D>
-__global__ void __launch_bounds__(32 * kWarps, 3) kv8_decode_kernel(const AttendArgs p) {
+template <int D, int RB>
+__global__ void __launch_bounds__(kThreads, RB == 1 ? 2 : 1)
+kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttendArgs p) {
+  constexpr int kRows = 8 * RB;
   constexpr int KC = D / 64;                     // 16-byte chunks of a key row per lane
-  constexpr int NT = D / 8;                      // n-tiles of the outputs
-  constexpr int VB = D / 8;                      // bytes of a value row per lane (columns c * VB ..)
-  __shared__ __align__(16) float s_o[kWarps][kRows][D];
+  constexpr int MT = D / 16;                     // 16-channel tiles of the outputs
+  constexpr int VB = D / 8;                      // bytes of a value row per lane (channels lr * VB ..)
+  using G = Ring<D>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const ring = smem_raw + (base - smem_u32(smem_raw));
+  auto full_bar = [&](int i) { return base + G::kStages * G::kStage + 8u * i; };
+  auto empty_bar = [&](int i) { return base + G::kStages * G::kStage + 8u * (G::kStages + i); };
+  uint4* const s_info = reinterpret_cast<uint4*>(ring + G::kStages * G::kStage + 16 * G::kStages);   // [stage], one word per 16 keys
+  float (*const s_o)[kRows][D] = reinterpret_cast<float (*)[kRows][D]>(ring);                       // [kWarps], when the ring is done with
+  static_assert(kWarps * kRows * D * 4 <= G::kStages * G::kStage, "the join reuses the ring");
+  __shared__ int s_abort;
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
   __shared__ int s_r[kWarps];
   __shared__ float s_cm[kRows], s_cl[kRows];     // this CTA's join
   __shared__ int s_cr;
 
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int i = 0; i < G::kStages; ++i) { mbar_init(full_bar(i), 1); mbar_init(empty_bar(i), 2); }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  __syncthreads();
+  volatile int* abort_flag = &s_abort;
   b2q_pdl_entry();
   cg::cluster_group cluster = cg::this_cluster();
   const int split = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const Batch& t = p.t;
-  const int head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, tq = lane & 3;
+  const int head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lr = lane >> 2, tq = lane & 3;
   const int unit = (int)(blockIdx.x / split);
   const bool tell = head == 0 && part == 0 && warp == 0;
 
@@ -87,201 +144,324 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv8_decode_kernel(const Attend
   const int64_t rows = (int64_t)r.n * p.group, row0 = (int64_t)f.y * kRows;
   const int valid = (int)min((int64_t)kRows, rows - row0);            // <= 0: an impossible sequence, its rows stay as they are
   if (valid <= 0) return;
-  const bool live = row < valid;
-  const int token = live ? (int)((row0 + row) / p.group) : 0;
-  const int qhead = head * p.group + (live ? (int)((row0 + row) % p.group) : 0);
-  const int pos = live ? r.len - r.n + token : -1;
   const int first_pos = r.len - r.n + (int)(row0 / p.group), last_pos = r.len - r.n + (int)((row0 + valid - 1) / p.group);
   const int key_end = last_pos + 1;
   const int key_begin = p.window > 0 ? max(0, first_pos - p.window + 1) & ~(kTile - 1) : 0;
 
-  // ---- the query rows as two E4M3 terms ----
-  uint32_t qa[2 * KC][4];
-  float qf;
-  {
-    const __nv_bfloat16* qp = p.q + (int64_t)(r.r0 + token) * p.ld_q + (int64_t)qhead * D + tq * 16;
-    uint4 w[KC][2];
-    float amax = 0.0f;
-    bool bad = false;
+  const int tiles = (key_end - key_begin + kTile - 1) / kTile, mine = (tiles - part + split - 1) / split;   // tiles part, part + split, ..
+
+  float o[RB][MT][4];
+  float m[RB][2], l[RB][2];
+  int R = kNone;
 #pragma unroll
-    for (int c = 0; c < KC; ++c)
+  for (int x = 0; x < RB; ++x) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        w[c][s] = live ? *reinterpret_cast<const uint4*>(qp + c * 64 + s * 8) : make_uint4(0, 0, 0, 0);
-        const uint32_t u[4] = {w[c][s].x, w[c][s].y, w[c][s].z, w[c][s].w};
+    for (int j = 0; j < MT; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a = fabsf(__uint_as_float(u[j] << 16)), b = fabsf(__uint_as_float(u[j] & 0xFFFF0000u));
-          bad |= !(a < INFINITY) || !(b < INFINITY);
-          amax = fmaxf(amax, fmaxf(a, b));
-        }
-      }
-    amax = quad_max(amax);
-    bad = (__ballot_sync(0xffffffffu, bad) >> (lane & 28)) & 0xF;
-    const uint32_t u = __float_as_uint(amax);
-    const int e = max(-119, (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0));
-    const float inv = pow2i(-e);
-    qf = bad ? __uint_as_float(0x7FC00000u) : p.scale * pow2i(e);
-#pragma unroll
-    for (int c = 0; c < KC; ++c)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const uint32_t uw[4] = {w[c][s].x, w[c][s].y, w[c][s].z, w[c][s].w};
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) split2(__uint_as_float(uw[j] << 16) * inv, __uint_as_float(uw[j] & 0xFFFF0000u) * inv, hi[j], lo[j]);
-        qa[2 * c + s][0] = hi[0] | (hi[1] << 16); qa[2 * c + s][1] = lo[0] | (lo[1] << 16);
-        qa[2 * c + s][2] = hi[2] | (hi[3] << 16); qa[2 * c + s][3] = lo[2] | (lo[3] << 16);
-      }
+      for (int i = 0; i < 4; ++i) o[x][j][i] = 0.0f;
+    m[x][0] = m[x][1] = -INFINITY;
+    l[x][0] = l[x][1] = 0.0f;
   }
 
-  float o[NT][4];
+  if (warp == kWarps) {
+    // ---------------- producer: the pages and scales of 32 tiles at a time, a tile to a lane, fetched while the copies of the 32 before
+    // them are issued ----------------
+    const int subs = t.page_shift >= 6 ? 1 : 64 >> t.page_shift, rows_each = kTile / subs;   // pages that a tile spans, their keys
+    int pg[4];
+    uint32_t info[4];
+    auto fetch = [&](int i0) {
+      const int j0 = key_begin + kTile * (part + split * (i0 + lane));
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+      for (int e = 0; e < 4; ++e) {
+        pg[e] = -1; info[e] = 0;
+        const int j = j0 + rows_each * e;
+        if (e < subs && i0 + lane < mine && j < key_end) {
+          pg[e] = page_of(t, f.x, j >> t.page_shift, head == 0);
+          if (pg[e] >= 0)
+            info[e] = 0x80000000u | (uint32_t)p.ks[(int64_t)pg[e] * t.n_kv_heads + head] | ((uint32_t)p.vs[(int64_t)pg[e] * t.n_kv_heads + head] << 8);
+        }
+      }
+    };
+    bool ok = true;
+    fetch(0);
+    for (int i0 = 0; i0 < mine && ok; i0 += 32) {
+      int cp[4];
+      uint32_t ci[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[j][i] = 0.0f;
-  float m = -INFINITY, l = 0.0f;
-  int R = kNone;
+      for (int e = 0; e < 4; ++e) { cp[e] = pg[e]; ci[e] = info[e]; }
+      if (i0 + 32 < mine) fetch(i0 + 32);
+      const int n = min(32, mine - i0);
+      for (int i = 0; i < n; ++i) {
+        const int it = i0 + i, st = it % G::kStages, j = key_begin + kTile * (part + split * it);
+        int p4[4];
+        uint32_t f4[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (e >= subs) { p4[e] = -1; f4[e] = 0; continue; }
+          p4[e] = __shfl_sync(0xffffffffu, cp[e], i); f4[e] = __shfl_sync(0xffffffffu, ci[e], i);
+        }
+        if (lane == 0) {
+          ok = mbar_wait_bounded(empty_bar(st), ((it / G::kStages) & 1) ^ 1, abort_flag, kWaitLimitNs, 1);
+          if (ok) {
+            s_info[st] = subs == 1 ? make_uint4(f4[0], f4[0], f4[0], f4[0]) : subs == 2 ? make_uint4(f4[0], f4[0], f4[1], f4[1]) : make_uint4(f4[0], f4[1], f4[2], f4[3]);
+            const int in_page = j & ((1 << t.page_shift) - 1);        // 0 but for pages of 128
+            int there = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) there += p4[e] >= 0;
+            const uint32_t dk = base + st * G::kStage, dv = dk + G::kHalf;
+            mbar_expect_tx(full_bar(st), (uint32_t)(there * rows_each) * 2 * D);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (p4[e] < 0) continue;
+              // the maps see lines of 128 bytes: one token of 128 channels, or two of 64
+              const int line = (((p4[e] * t.n_kv_heads + head) << t.page_shift) + in_page) / (128 / D);
+              tma_load_2d(dk + e * rows_each * D, &map_k, full_bar(st), 0, line);
+              tma_load_2d(dv + e * rows_each * D, &map_v, full_bar(st), 0, line);
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+      }
+    }
+    if (!ok && lane == 0) {                      // give copies in flight time to land before shared memory is released
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 2000000ull) {}
+    }
+  } else {
+    // ---- the query rows: this lane holds channels 64 c + 16 tq .. of rows lr, lr + 8, .. as the 8-column operand ----
+    uint32_t qb[RB][4 * KC][2];
+    float qf[RB][2];                               // score factors of rows 8 x + 2 tq + {0, 1}, the rows of this lane's scores
+    int pos[RB][2];
+#pragma unroll
+    for (int x = 0; x < RB; ++x) {
+      const int row = 8 * x + lr;
+      const bool live = row < valid;
+      const int token = live ? (int)((row0 + row) / p.group) : 0, g = live ? (int)((row0 + row) % p.group) : 0;
+      const __nv_bfloat16* qp = p.q + (int64_t)(r.r0 + token) * p.ld_q + (int64_t)(head * p.group + g) * D + tq * 16;
+      uint4 w[KC][2];
+      float amax = 0.0f;
+      bool bad = false;
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          w[c][s] = live ? *reinterpret_cast<const uint4*>(qp + c * 64 + s * 8) : make_uint4(0, 0, 0, 0);
+          const uint32_t u[4] = {w[c][s].x, w[c][s].y, w[c][s].z, w[c][s].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float a = fabsf(__uint_as_float(u[j] << 16)), b = fabsf(__uint_as_float(u[j] & 0xFFFF0000u));
+            bad |= !(a < INFINITY) || !(b < INFINITY);
+            amax = fmaxf(amax, fmaxf(a, b));
+          }
+        }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      bad = (__ballot_sync(0xffffffffu, bad) >> (lane & 28)) & 0xF;
+      const int e = max(-126, (int)(__float_as_uint(amax) >> 23) - 127 - 14);
+      const float inv = p.scale < 0.0f ? -pow2i(-e) : pow2i(-e);        // a negative scale enters with the query
+      const float factor = bad ? __uint_as_float(0x7FC00000u) : fabsf(p.scale) * pow2i(e);   // a query with an infinity or a NaN: NaN throughout
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const uint32_t u[4] = {w[c][s].x, w[c][s].y, w[c][s].z, w[c][s].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            qb[x][4 * c + 2 * s + (j >> 1)][j & 1] = pack_f16(__uint_as_float(u[j] << 16) * inv, __uint_as_float(u[j] & 0xFFFF0000u) * inv);
+        }
+#pragma unroll
+      for (int e2 = 0; e2 < 2; ++e2) {
+        qf[x][e2] = __shfl_sync(0xffffffffu, factor, 8 * tq + 4 * e2);
+        const int rr = 8 * x + 2 * tq + e2;
+        pos[x][e2] = rr < valid ? r.len - r.n + (int)((row0 + rr) / p.group) : -1;
+      }
+    }
 
-  const int step = kTile * kWarps * split;
-  // page and scales of the 8-key group lane & 3 of a tile (a group never crosses a page)
-  auto fetch = [&](int j0, int& pg, uint32_t& sc) {
-    pg = -1; sc = 0;
-    const int j = j0 + 8 * tq;
-    if (j < key_end) {
-      pg = page_of(t, f.x, j >> t.page_shift, head == 0);
-      if (pg >= 0) sc = (uint32_t)p.ks[(int64_t)pg * t.n_kv_heads + head] | ((uint32_t)p.vs[(int64_t)pg * t.n_kv_heads + head] << 8);
-    }
-  };
-  int j0 = key_begin + kTile * (part * kWarps + warp);
-  int npg; uint32_t nsc;
-  fetch(j0, npg, nsc);
-  for (; j0 < key_end; j0 += step) {
-    int pg[4]; uint32_t sc[4];
+    const int mk = key_of<D>(lr), ve[2] = {key_of<D>(2 * tq), key_of<D>(2 * tq + 1)};   // this lane's key row, its two value rows (mod 8)
+    for (int it = warp >> 1; it < mine; it += kWarps / 2) {
+      const int st = it % G::kStages, j0 = key_begin + kTile * (part + split * it) + 32 * (warp & 1);   // this warp's 32 keys
+      if (!mbar_wait_bounded(full_bar(st), (it / G::kStages) & 1, abort_flag, kWaitLimitNs, 1)) break;
+      __syncwarp();
+      const uint8_t* const ks = ring + st * G::kStage + 32 * (warp & 1) * D;
+      uint8_t* const vs = ring + st * G::kStage + G::kHalf + 32 * (warp & 1) * D;
+      const uint2 info = reinterpret_cast<const uint2*>(s_info + st)[warp & 1];
+      const uint32_t sc[2] = {info.x, info.y};     // of keys 0..15 and 16..31
+      if (j0 < key_end) {
+        // whole: every key is there; clear: and every row sees every key, under one pair of scales
+        const bool whole = (sc[0] & sc[1]) >> 31 && j0 + 32 <= key_end;
+        const bool clear = whole && sc[0] == sc[1] && j0 + 31 <= first_pos && (p.window <= 0 || j0 > last_pos - p.window);
+        if (!whole) {                              // value rows without a visible key: whatever they hold becomes 0
+          if (!(sc[lane >> 4] >> 31) || j0 + lane >= key_end)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) { pg[g] = __shfl_sync(0xffffffffu, npg, g); sc[g] = __shfl_sync(0xffffffffu, nsc, g); }
-    uint4 kr[4][KC];
+            for (int u = 0; u < D / 16; ++u) *reinterpret_cast<uint4*>(vs + swz<D>(lane, u)) = make_uint4(0, 0, 0, 0);
+          __syncwarp();
+        }
+
+        // ---- products with the keys: this lane has keys j0 + 8 g + mk of rows 8 x + 2 tq + {0, 1} ----
+        float s[RB][4][2];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int j = j0 + 8 * g + row;
-      const bool in = pg[g] >= 0 && j < key_end;
-      const uint8_t* kp = p.k + (((((int64_t)pg[g] * t.n_kv_heads + head) << t.page_shift) + (j & ((1 << t.page_shift) - 1))) * D) + tq * 16;
+        for (int mt = 0; mt < 2; ++mt) {
+          float c[RB][4];
 #pragma unroll
-      for (int c = 0; c < KC; ++c) kr[g][c] = in ? ld_stream(kp + c * 64) : make_uint4(0, 0, 0, 0);
-    }
-    uint32_t vr[4][2][VB / 4];
+          for (int x = 0; x < RB; ++x)
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
+            for (int i = 0; i < 4; ++i) c[x][i] = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int j = j0 + 8 * g + 2 * tq + e;
-        const bool in = pg[g] >= 0 && j < key_end;
-        const uint8_t* vp = p.v + (((((int64_t)pg[g] * t.n_kv_heads + head) << t.page_shift) + (j & ((1 << t.page_shift) - 1))) * D) + row * VB;
-        if constexpr (D == 128) {
-          const uint4 x = in ? ld_stream(vp) : make_uint4(0, 0, 0, 0);
-          vr[g][e][0] = x.x; vr[g][e][1] = x.y; vr[g][e][2] = x.z; vr[g][e][3] = x.w;
+          for (int ch = 0; ch < KC; ++ch) {
+            const uint4 k0 = *reinterpret_cast<const uint4*>(ks + swz<D>(16 * mt + mk, 4 * ch + tq));
+            const uint4 k1 = *reinterpret_cast<const uint4*>(ks + swz<D>(16 * mt + 8 + mk, 4 * ch + tq));
+            const uint32_t ka[4] = {k0.x, k0.y, k0.z, k0.w}, kb[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t a0, a1, a2, a3;
+              to_f16(ka[k], a0, a2);
+              to_f16(kb[k], a1, a3);
+#pragma unroll
+              for (int x = 0; x < RB; ++x) mma_f16(c[x], a0, a1, a2, a3, qb[x][4 * ch + k][0], qb[x][4 * ch + k][1]);
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < RB; ++x)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) s[x][2 * mt + h][e] = c[x][2 * h + e];
+        }
+        uint32_t vr[4][2][VB / 4];                 // values of keys 8 g + ve[e], channels VB lr ..
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if constexpr (D == 128) {
+              const uint4 x = *reinterpret_cast<const uint4*>(vs + swz<D>(8 * g + ve[e], lr));
+              vr[g][e][0] = x.x; vr[g][e][1] = x.y; vr[g][e][2] = x.z; vr[g][e][3] = x.w;
+            } else {
+              const uint2 x = *reinterpret_cast<const uint2*>(vs + swz<D>(8 * g + ve[e], lr >> 1) + 8 * (lr & 1));
+              vr[g][e][0] = x.x; vr[g][e][1] = x.y;
+            }
+          }
+        // o = a * o + P^T V with pb: keys 8 g + ve[e] of row 8 x + lr
+        auto accumulate = [&](const float (&a)[RB][2], const uint32_t (&pb)[RB][4]) {
+          bool moved = false;
+#pragma unroll
+          for (int x = 0; x < RB; ++x) moved |= a[x][0] != 1.0f || a[x][1] != 1.0f;
+          if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int x = 0; x < RB; ++x)
+#pragma unroll
+              for (int j = 0; j < MT; ++j) { o[x][j][0] *= a[x][0]; o[x][j][1] *= a[x][1]; o[x][j][2] *= a[x][0]; o[x][j][3] *= a[x][1]; }
+          }
+#pragma unroll
+          for (int w = 0; w < VB / 4; ++w) {                            // channels VB lr + 4 w .. + 3: two tiles of 16
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              const int sel = hf ? 0x7362 : 0x5140;                     // channel pairs of two keys: k0 c0, k1 c0, k0 c1, k1 c1
+#pragma unroll
+              for (int k2 = 0; k2 < 2; ++k2) {
+                uint32_t a0, a1, a2, a3;
+                to_f16(__byte_perm(vr[2 * k2][0][w], vr[2 * k2][1][w], sel), a0, a1);
+                to_f16(__byte_perm(vr[2 * k2 + 1][0][w], vr[2 * k2 + 1][1][w], sel), a2, a3);
+#pragma unroll
+                for (int x = 0; x < RB; ++x) mma_f16(o[x][2 * w + hf], a0, a1, a2, a3, pb[x][2 * k2], pb[x][2 * k2 + 1]);
+              }
+            }
+          }
+        };
+        const int lv[2] = {(int)(sc[0] >> 8 & 0xFF) - 127, (int)(sc[1] >> 8 & 0xFF) - 127};
+        float alpha[RB][2];
+        uint32_t pb[RB][4];
+        if (clear) {
+          const int was = R == kNone ? lv[0] : R;
+          R = lv[0] > was || lv[0] < was - kSpan ? lv[0] : was;
+          const float kf = pow2_byte(sc[0] & 0xFF), move = pow2i(was - R), down = pow2i(R - lv[0] - 15), shift = (float)(15 + lv[0] - R);
+#pragma unroll
+          for (int x = 0; x < RB; ++x) {
+            float w[4][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float fs = qf[x][e] * kf;                           // not negative: the sign of the scale is in the query
+              const float mn = fmaxf(m[x][e], column_max(fmaxf(fmaxf(s[x][0][e], s[x][1][e]), fmaxf(s[x][2][e], s[x][3][e]))) * fs);
+              const float a = ex2(m[x][e] - mn), base = shift - mn;
+              alpha[x][e] = a * move;
+              m[x][e] = mn;
+              float sum = 0.0f;
+#pragma unroll
+              for (int g = 0; g < 4; ++g) { w[g][e] = ex2(fmaf(s[x][g][e], fs, base)); sum += w[g][e]; }
+              l[x][e] = fmaf(l[x][e], a, sum * down);                   // the sum is of the weights without the values' scale
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) pb[x][g] = transpose8x8(pack_f16(w[g][0], w[g][1]));
+          }
+          accumulate(alpha, pb);
         } else {
-          const uint2 x = in ? __ldcs(reinterpret_cast<const uint2*>(vp)) : make_uint2(0, 0);
-          vr[g][e][0] = x.x; vr[g][e][1] = x.y;
+#pragma unroll
+          for (int x = 0; x < RB; ++x)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mt = -INFINITY;
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const int j = j0 + 8 * g + mk;
+                const bool see = j <= pos[x][e] && (p.window <= 0 || j > pos[x][e] - p.window) && sc[g >> 1] >> 31;
+                s[x][g][e] = see ? s[x][g][e] * (qf[x][e] * pow2_byte(sc[g >> 1] & 0xFF)) : -INFINITY;
+                mt = fmaxf(mt, s[x][g][e]);
+              }
+              const float mn = fmaxf(m[x][e], column_max(mt)), base = mn == -INFINITY ? 0.0f : mn;   // nothing seen yet: exp2(-inf - 0) = 0
+              alpha[x][e] = ex2(m[x][e] - base);
+              m[x][e] = mn;
+              l[x][e] *= alpha[x][e];
+#pragma unroll
+              for (int g = 0; g < 4; ++g) { s[x][g][e] = ex2(s[x][g][e] - base); l[x][e] += s[x][g][e]; }
+            }
+          // the halves whose value scales lie within 2^kSpan of the larger together, else one after the other
+          unsigned rem = (sc[0] >> 31) | (sc[1] >> 31 && j0 + 16 < key_end ? 2u : 0u);
+          while (rem) {
+            const int lead = rem == 3 ? max(lv[0], lv[1]) : rem == 1 ? lv[0] : lv[1];
+            const unsigned take = rem & ((lv[0] >= lead - kSpan ? 1u : 0u) | (lv[1] >= lead - kSpan ? 2u : 0u));
+            const int was = R == kNone ? lead : R;
+            R = lead > was || lead < was - kSpan ? lead : was;
+            const float move = pow2i(was - R), up[2] = {take & 1 ? pow2i(15 + lv[0] - R) : 0.0f, take & 2 ? pow2i(15 + lv[1] - R) : 0.0f};
+#pragma unroll
+            for (int x = 0; x < RB; ++x) {
+              alpha[x][0] *= move; alpha[x][1] *= move;
+#pragma unroll
+              for (int g = 0; g < 4; ++g) pb[x][g] = transpose8x8(pack_f16(s[x][g][0] * up[g >> 1], s[x][g][1] * up[g >> 1]));
+            }
+            accumulate(alpha, pb);
+#pragma unroll
+            for (int x = 0; x < RB; ++x) alpha[x][0] = alpha[x][1] = 1.0f;
+            rem &= ~take;
+          }
         }
+        if (!whole) fence_async_smem();            // the zeros, before the next copy into this stage
       }
-    fetch(j0 + step, npg, nsc);
-
-    // ---- scores of 8 rows x 32 keys: this lane has keys j0 + 8 g + 2 tq + {0, 1} of its row ----
-    float s[4][2], mt = -INFINITY;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int x = 0; x < KC; ++x) {
-        mma_e4m3(c, qa[2 * x][0], qa[2 * x][1], qa[2 * x][2], qa[2 * x][3], kr[g][x].x, kr[g][x].y);
-        mma_e4m3(c, qa[2 * x + 1][0], qa[2 * x + 1][1], qa[2 * x + 1][2], qa[2 * x + 1][3], kr[g][x].z, kr[g][x].w);
-      }
-      const float kf = qf * pow2_byte(sc[g] & 0xFF);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int j = j0 + 8 * g + 2 * tq + e;
-        const bool see = j <= pos && (p.window <= 0 || j > pos - p.window) && pg[g] >= 0;
-        s[g][e] = see ? (c[e] + c[2 + e]) * kf : -INFINITY;
-        mt = fmaxf(mt, s[g][e]);
-      }
-    }
-    const float mn = fmaxf(m, quad_max(mt));
-    const float base = mn == -INFINITY ? 0.0f : mn;                   // a row that has seen nothing yet: exp2(-inf - 0) = 0
-    float alpha = exp2f(m - base);
-    m = mn;
-    l *= alpha;
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) { s[g][e] = exp2f(s[g][e] - base); l += s[g][e]; }
-
-    // ---- outputs: the groups whose value scales lie within 2^4 of the largest at a time (nearly always all of them) ----
-    unsigned rem = 0;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) rem |= (pg[g] >= 0 && j0 + 8 * g < key_end) ? 1u << g : 0u;
-    while (rem) {
-      int lead = kNone;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) if (rem >> g & 1) lead = max(lead, (int)(sc[g] >> 8) - 127);
-      unsigned take = 0;
-      if (R == kNone) R = lead;
-      const int was = R;
-      R = lead > R || lead < R - 4 ? lead : R;
-      alpha *= pow2i(was - R);
-      float w[4][2];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int lv = (int)(sc[g] >> 8) - 127;
-        const bool on = (rem >> g & 1) && lv >= lead - 4;
-        take |= on ? 1u << g : 0u;
-        const float up = on ? pow2i(8 + lv - R) : 0.0f;
-        w[g][0] = s[g][0] * up; w[g][1] = s[g][1] * up;
-      }
-      rem &= ~take;
-      if (__any_sync(0xffffffffu, alpha != 1.0f)) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[j][i] *= alpha;
-        alpha = 1.0f;
-      }
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) split2(w[g][0], w[g][1], hi[g], lo[g]);
-      const uint32_t a0 = hi[0] | (hi[1] << 16), a1 = lo[0] | (lo[1] << 16), a2 = hi[2] | (hi[3] << 16), a3 = lo[2] | (lo[3] << 16);
-#pragma unroll
-      for (int x = 0; x < VB / 4; ++x) {                              // 4 columns at a time: 4 x 4 byte transposes
-        uint32_t b[2][4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t r0 = vr[2 * h][0][x], r1 = vr[2 * h][1][x], r2 = vr[2 * h + 1][0][x], r3 = vr[2 * h + 1][1][x];
-          const uint32_t t0 = __byte_perm(r0, r1, 0x5140), t1 = __byte_perm(r0, r1, 0x7362), t2 = __byte_perm(r2, r3, 0x5140), t3 = __byte_perm(r2, r3, 0x7362);
-          b[h][0] = __byte_perm(t0, t2, 0x5410); b[h][1] = __byte_perm(t0, t2, 0x7632);
-          b[h][2] = __byte_perm(t1, t3, 0x5410); b[h][3] = __byte_perm(t1, t3, 0x7632);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mma_e4m3(o[4 * x + i], a0, a1, a2, a3, b[0][i], b[1][i]);
-      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty_bar(st));
     }
   }
 
   // ---- join the warps of this CTA, then the CTAs of the cluster ----
-  l += __shfl_xor_sync(0xffffffffu, l, 1);
-  l += __shfl_xor_sync(0xffffffffu, l, 2);
-  if (tq == 0) { s_m[warp][row] = m; s_l[warp][row] = l; }
-  if (lane == 0) s_r[warp] = R;
+  __syncthreads();                               // every tile has been multiplied: the ring is free
+  if (warp < kWarps) {
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
+    for (int x = 0; x < RB; ++x)
 #pragma unroll
-    for (int j = 0; j < NT; j += 4)                                   // columns (2 tq + e) * VB + j ..
-      *reinterpret_cast<float4*>(&s_o[warp][row][(2 * tq + e) * VB + j]) =
-          make_float4(o[j][e] + o[j][2 + e], o[j + 1][e] + o[j + 1][2 + e], o[j + 2][e] + o[j + 2][2 + e], o[j + 3][e] + o[j + 3][2 + e]);
+      for (int e = 0; e < 2; ++e) {
+        const float ll = column_sum(l[x][e]);
+        const int rr = 8 * x + 2 * tq + e;
+        if (lr == 0) { s_m[warp][rr] = m[x][e]; s_l[warp][rr] = ll; }
+#pragma unroll
+        for (int j = 0; j < MT; j += 2)                                 // tile j: channels VB lr + 2 j + {0, 1} (registers e and 2 + e)
+          *reinterpret_cast<float4*>(&s_o[warp][rr][lr * VB + 2 * j]) = make_float4(o[x][j][e], o[x][j][2 + e], o[x][j + 1][e], o[x][j + 1][2 + e]);
+      }
+    if (lane == 0) s_r[warp] = R;
+  }
   __syncthreads();
   int cr = kNone;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) cr = max(cr, s_r[w]);
-  for (int i = threadIdx.x; i < kRows * D / 4; i += 32 * kWarps) {
+  for (int i = threadIdx.x; i < kRows * D / 4; i += kThreads) {
     const int rr = i / (D / 4), cc = (i % (D / 4)) * 4;
     float mm = -INFINITY, ll = 0.0f;
 #pragma unroll
@@ -290,7 +470,7 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv8_decode_kernel(const Attend
     float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float a = exp2f(s_m[w][rr] - b), fo = a * (s_r[w] == kNone ? 0.0f : pow2i(s_r[w] - cr));
+      const float a = ex2(s_m[w][rr] - b), fo = a * (s_r[w] == kNone ? 0.0f : pow2i(s_r[w] - cr));
       ll += a * s_l[w][rr];
       const float4 x = *reinterpret_cast<const float4*>(&s_o[w][rr][cc]);
       acc.x += fo * x.x; acc.y += fo * x.y; acc.z += fo * x.z; acc.w += fo * x.w;
@@ -302,8 +482,8 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv8_decode_kernel(const Attend
   if (split > 1) cluster.sync(); else __syncthreads();
   int tr = kNone;
   for (int c = 0; c < split; ++c) tr = max(tr, split > 1 ? *cluster.map_shared_rank(&s_cr, c) : s_cr);
-  const int cols = D / split;                                         // this CTA finishes columns part * cols ..
-  for (int i = threadIdx.x; i < kRows * cols / 4; i += 32 * kWarps) {
+  const int cols = D / split;                                         // this CTA finishes channels part * cols ..
+  for (int i = threadIdx.x; i < kRows * cols / 4; i += kThreads) {
     const int rr = i / (cols / 4), cc = part * cols + (i % (cols / 4)) * 4;
     if (rr >= valid) continue;
     float mm = -INFINITY, ll = 0.0f;
@@ -311,7 +491,7 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv8_decode_kernel(const Attend
     const float b = mm == -INFINITY ? 0.0f : mm;
     float4 acc = make_float4(0, 0, 0, 0);
     for (int c = 0; c < split; ++c) {
-      const float a = exp2f((split > 1 ? *cluster.map_shared_rank(&s_cm[rr], c) : s_cm[rr]) - b);
+      const float a = ex2((split > 1 ? *cluster.map_shared_rank(&s_cm[rr], c) : s_cm[rr]) - b);
       const int rc = split > 1 ? *cluster.map_shared_rank(&s_cr, c) : s_cr;
       const float fo = a * (rc == kNone ? 0.0f : pow2i(rc - tr));
       ll += a * (split > 1 ? *cluster.map_shared_rank(&s_cl[rr], c) : s_cl[rr]);
@@ -319,25 +499,36 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv8_decode_kernel(const Attend
       acc.x += fo * x.x; acc.y += fo * x.y; acc.z += fo * x.z; acc.w += fo * x.w;
     }
     const int tk = (int)((row0 + rr) / p.group), hd = head * p.group + (int)((row0 + rr) % p.group);
-    const int64_t orow2 = (int64_t)(r.r0 + tk) * (t.n_kv_heads * p.group) + hd;
+    const int64_t orow = (int64_t)(r.r0 + tk) * (t.n_kv_heads * p.group) + hd;
     // a row that sees no key has ll = 0: zeros and -inf.  A query that holds an infinity or a NaN has ll = NaN and stays NaN.
-    const float inv = ll == 0.0f ? 0.0f : __frcp_rn(ll), up = tr == kNone ? 0.0f : pow2i(tr - 8);
+    const float inv = ll == 0.0f ? 0.0f : __frcp_rn(ll), up = tr == kNone ? 0.0f : pow2i(tr - 15);
     const __nv_bfloat162 y0 = __floats2bfloat162_rn(acc.x * inv * up, acc.y * inv * up), y1 = __floats2bfloat162_rn(acc.z * inv * up, acc.w * inv * up);
     uint2 pk;
     pk.x = *reinterpret_cast<const uint32_t*>(&y0); pk.y = *reinterpret_cast<const uint32_t*>(&y1);
-    *reinterpret_cast<uint2*>(p.out + orow2 * D + cc) = pk;
-    if (p.lse && cc == 0) p.lse[orow2] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
+    *reinterpret_cast<uint2*>(p.out + orow * D + cc) = pk;
+    if (p.lse && cc == 0) p.lse[orow] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
   }
   if (split > 1) cluster.sync();                                      // the others may still be reading this CTA's shared memory
+  if (threadIdx.x == 0 && s_abort) report(t.status, B2Q_ERR_TIMEOUT);
 }
 
 }  // namespace kv8
 
-template <int D>
+template <int D, int RB>
 static int32_t kv8_decode_launch(b2q_handle h, const kv8::AttendArgs& p, int64_t units, int split) {
+  using G = kv8::Ring<D>;
+  CUtensorMap map_k, map_v;
+  const uint64_t lines = ((uint64_t)p.t.num_pages * p.t.n_kv_heads << p.t.page_shift) / (128 / D);
+  const uint32_t box = (p.t.page_shift < 6 ? 1 << p.t.page_shift : kv8::kTile) / (128 / D);
+  int32_t st = b2q_tensor_map_2d(h, &map_k, p.k, 1, 128, lines, 128, box);
+  if (st != B2Q_OK) return st;
+  st = b2q_tensor_map_2d(h, &map_v, p.v, 1, 128, lines, 128, box);
+  if (st != B2Q_OK) return st;
+  B2Q_SMEM_ATTR(h, (kv8::kv8_decode_kernel<D, RB>), G::kSmem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * split), (unsigned)p.t.n_kv_heads);
-  cfg.blockDim = dim3(32 * kv8::kWarps);
+  cfg.blockDim = dim3(kv8::kThreads);
+  cfg.dynamicSmemBytes = G::kSmem;
   cfg.stream = h->stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -348,7 +539,7 @@ static int32_t kv8_decode_launch(b2q_handle h, const kv8::AttendArgs& p, int64_t
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = h->sw.chain_pdl != 0 ? 2 : 1;
-  B2Q_CUDA(h, cudaLaunchKernelEx(&cfg, kv8::kv8_decode_kernel<D>, p));
+  B2Q_CUDA(h, cudaLaunchKernelEx(&cfg, (kv8::kv8_decode_kernel<D, RB>), map_k, map_v, p));
   return B2Q_OK;
 }
 
@@ -375,10 +566,13 @@ extern "C" int32_t b2q_kv8_attention_bf16(b2q_handle h, const void* q, int64_t l
   p.window = window > 0 && window < most ? (int)window : 0;
   p.scale = scale * 1.4426950408889634f;
   p.out = static_cast<__nv_bfloat16*>(out); p.lse = lse;
-  const int64_t units = q_starts ? tokens * p.group / kv8::kRows + seqs : seqs * ceil_div64(p.group, kv8::kRows);
+  // rows that share keys: up to 8 a CTA, 16 where a sequence has more than 8 on average (one conversion of the codes serves both halves)
+  const int rb = tokens * p.group > 8 * seqs ? 2 : 1, per = 8 * rb;
+  const int64_t units = q_starts ? tokens * p.group / per + seqs : seqs * ceil_div64(p.group, per);
   const int64_t keys = p.window ? p.window + kv8::kTile : most;
   int split = 1;
-  while (split < 8 && units * n_kv_heads * split * 2 <= 3 * (int64_t)h->sm_count && keys > split * kv8::kTile * kv8::kWarps) split *= 2;
+  while (split < 8 && units * n_kv_heads * split * 2 <= 4 * (int64_t)h->sm_count && keys > split * kv8::kTile * kv8::kWarps / 2) split *= 2;
   if (units * split > 0x7FFFFFFF) B2Q_FAIL(h, B2Q_ERR_INVALID_DIMENSION, "kv8_attention: %lld tokens of %lld heads are too many", (long long)tokens, (long long)n_heads);
-  return head_dim == 64 ? kv8_decode_launch<64>(h, p, units, split) : kv8_decode_launch<128>(h, p, units, split);
+  if (head_dim == 64) return rb == 1 ? kv8_decode_launch<64, 1>(h, p, units, split) : kv8_decode_launch<64, 2>(h, p, units, split);
+  return rb == 1 ? kv8_decode_launch<128, 1>(h, p, units, split) : kv8_decode_launch<128, 2>(h, p, units, split);
 }
