@@ -29,10 +29,10 @@ int32_t b2q_workspace2(b2q_handle h, size_t bytes, void** out) {
   return B2Q_OK;
 }
 
-int32_t b2q_tensor_map_2d(b2q_handle h, CUtensorMap* map, const void* ptr, int elem_bytes, uint64_t d0, uint64_t d1, uint32_t box0,
-                          uint32_t box1) {
+static int32_t tensor_map_2d(b2q_handle h, CUtensorMap* map, const void* ptr, int elem_bytes, uint64_t d0, uint64_t d1, uint32_t box0,
+                             uint32_t box1, CUtensorMapSwizzle swizzle) {
   static_assert(sizeof(CUtensorMap) == 128, "CUtensorMap size");
-  const uint64_t key[4] = {(uint64_t)reinterpret_cast<uintptr_t>(ptr), d0, d1, ((uint64_t)box0 << 40) | ((uint64_t)box1 << 8) | (uint64_t)elem_bytes};
+  const uint64_t key[4] = {(uint64_t)reinterpret_cast<uintptr_t>(ptr), d0, d1, ((uint64_t)box0 << 40) | ((uint64_t)box1 << 8) | ((uint64_t)swizzle << 4) | (uint64_t)elem_bytes};
   uint64_t hsh = key[0] * 0x9E3779B97F4A7C15ull ^ key[1] * 0xC2B2AE3D27D4EB4Full ^ key[2] * 0x165667B19E3779F9ull ^ key[3];
   hsh ^= hsh >> 29;
   b2q_handle_s::MapEntry* e = h->map_cache ? &h->map_cache[hsh % kMapCacheEntries] : nullptr;
@@ -48,7 +48,7 @@ int32_t b2q_tensor_map_2d(b2q_handle h, CUtensorMap* map, const void* ptr, int e
   cuuint32_t estr[2] = {1, 1};
   const CUtensorMapDataType dt = elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-  CUresult r = enc(map, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  CUresult r = enc(map, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) B2Q_FAIL(h, B2Q_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
   if (e) {
@@ -57,6 +57,14 @@ int32_t b2q_tensor_map_2d(b2q_handle h, CUtensorMap* map, const void* ptr, int e
     e->valid = 1;
   }
   return B2Q_OK;
+}
+
+int32_t b2q_tensor_map_2d(b2q_handle h, CUtensorMap* map, const void* ptr, int elem_bytes, uint64_t d0, uint64_t d1, uint32_t box0,
+                          uint32_t box1) {
+  return tensor_map_2d(h, map, ptr, elem_bytes, d0, d1, box0, box1, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+int32_t b2q_tensor_map_2d_sw64(b2q_handle h, CUtensorMap* map, const void* ptr, uint64_t d0, uint64_t d1, uint32_t box1) {
+  return tensor_map_2d(h, map, ptr, 1, d0, d1, 64u, box1, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 extern "C" {

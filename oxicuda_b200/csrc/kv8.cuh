@@ -70,6 +70,18 @@ __device__ __forceinline__ int2 find_unit(int seqs, int64_t unit, F count) {
   return make_int2(-1, 0);
 }
 
+struct AttendArgs {
+  Batch t;
+  const __nv_bfloat16* q; int64_t ld_q;
+  const uint8_t* k; const uint8_t* v; const uint8_t* ks; const uint8_t* vs;
+  int group;                                     // query heads per kv head
+  int window;                                    // 0: none
+  float scale;                                   // softmax scale * log2(e)
+  __nv_bfloat16* out; float* lse;                // [tokens][heads][head_dim], [tokens][heads]
+};
+
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(min(127, max(-126, e)) + 127) << 23); }
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float pow2_byte(uint32_t e8m0) { return e8m0_to_f32_dev(e8m0); }
 
 }  // namespace kv8

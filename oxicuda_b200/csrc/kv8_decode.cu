@@ -44,16 +44,6 @@ template <int D> struct Ring {
 constexpr int kNone = -1000;                     // R of a warp that has seen no page
 constexpr int kSpan = 8;                         // value scales that share a product differ by at most 2^kSpan
 
-struct AttendArgs {
-  Batch t;
-  const __nv_bfloat16* q; int64_t ld_q;
-  const uint8_t* k; const uint8_t* v; const uint8_t* ks; const uint8_t* vs;
-  int group;                                     // query heads per kv head
-  int window;                                    // 0: none
-  float scale;                                   // softmax scale * log2(e)
-  __nv_bfloat16* out; float* lse;                // [tokens][heads][head_dim], [tokens][heads]
-};
-
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -82,8 +72,6 @@ __device__ __forceinline__ float column_sum(float v) {
   for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(min(127, max(-126, e)) + 127) << 23); }
-__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 // byte offset of 16-byte unit u of row r in a tile of D-byte rows whose 128-byte lines TMA has swizzled
 template <int D> __device__ __forceinline__ uint32_t swz(int r, int u) {
   const uint32_t at = (uint32_t)(r * D + u * 16);
@@ -543,6 +531,8 @@ static int32_t kv8_decode_launch(b2q_handle h, const kv8::AttendArgs& p, int64_t
   return B2Q_OK;
 }
 
+int32_t b2q_kv8_prefill(b2q_handle h, const kv8::AttendArgs& p, int64_t head_dim);   // kv8_prefill.cu
+
 extern "C" int32_t b2q_kv8_attention_bf16(b2q_handle h, const void* q, int64_t ld_q, int64_t tokens, int64_t n_heads, const int32_t* q_starts,
                                           const int32_t* seq_lens, const int32_t* block_tables, int64_t seqs, int64_t table_width, int64_t num_pages,
                                           int64_t page_size, int64_t n_kv_heads, int64_t head_dim, const uint8_t* k_codes, const uint8_t* v_codes,
@@ -566,6 +556,7 @@ extern "C" int32_t b2q_kv8_attention_bf16(b2q_handle h, const void* q, int64_t l
   p.window = window > 0 && window < most ? (int)window : 0;
   p.scale = scale * 1.4426950408889634f;
   p.out = static_cast<__nv_bfloat16*>(out); p.lse = lse;
+  if (q_starts && tokens * p.group > 32 * seqs) return b2q_kv8_prefill(h, p, head_dim);
   // rows that share keys: up to 8 a CTA, 16 where a sequence has more than 8 on average (one conversion of the codes serves both halves)
   const int rb = tokens * p.group > 8 * seqs ? 2 : 1, per = 8 * rb;
   const int64_t units = q_starts ? tokens * p.group / per + seqs : seqs * ceil_div64(p.group, per);
