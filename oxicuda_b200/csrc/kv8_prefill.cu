@@ -71,6 +71,15 @@ __device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, ui
 __device__ __forceinline__ void to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
+// two f16 -> two E4M3 codes, and the codes of what that leaves (exact in f16)
+__device__ __forceinline__ void split_f16(uint32_t x, uint16_t& hi, uint16_t& lo) {
+  asm("{\n\t.reg .b16 h;\n\t.reg .b32 b, r;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 h, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 b, h;\n\t"
+      "sub.rn.f16x2 r, %2, b;\n\t"
+      "mov.b16 %0, h;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 %1, r;\n\t}" : "=h"(hi), "=h"(lo) : "r"(x));
+}
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -102,7 +111,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   Info* const s_info = reinterpret_cast<Info*>(smem + (bar_at - base) + 8 * (2 * kKStages + 2 * kVStages + 10));
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
-  __shared__ float s_m[kRows], s_l[kRows];        // the join: this CTA's maxima, sums and units
+  __shared__ float s_m[kRows], s_l[kRows];        // score factors of the rows; for the join this CTA's maxima, sums and units
   __shared__ int s_r[kRows];
 
   cg::cluster_group cluster = cg::this_cluster();
@@ -133,7 +142,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   const Rows r = rows_of(t, f.x, false);
   const int64_t row0 = (int64_t)(count(f.x) - 1 - f.y) * kRows;
   const int valid = (int)min((int64_t)kRows, (int64_t)r.n * p.group - row0);
-  const int first_pos = r.len - r.n + (int)(row0 / p.group), last_pos = r.len - r.n + (int)((row0 + valid - 1) / p.group);
+  const int token0 = (int)(row0 / p.group), head0 = (int)(row0 - (int64_t)token0 * p.group);   // of the tile's first row, within the sequence and the group
+  const int first_pos = r.len - r.n + token0, last_pos = first_pos + (head0 + valid - 1) / p.group;
   const int key_end = last_pos + 1;
   const int key_begin = p.window > 0 ? max(0, first_pos - p.window + 1) & ~(kTile - 1) : 0;
   const int all = (key_end - key_begin + kTile - 1) / kTile, tiles = (all - part + split - 1) / split;   // tiles part, part + split, ..
@@ -298,6 +308,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       const int src0 = key0 * D + ((D == 128 ? u ^ (key0 & 7) : u ^ ((key0 >> 1) & 3)) << 4);              // as TMA left it
       const int dst0 = (u >> 2) * (kTile * 128) + key0 * 128 + ((u2 ^ (key0 & 7)) << 4);                   // block u / 4, units 2 (u & 3) and the next
       const int step = (((u2 + 1) ^ (key0 & 7)) - (u2 ^ (key0 & 7))) * 16;
+      if (wait(qready, 0))                          // the query rows have passed through the tiles that are written here
       for (int it = 0;; ++it) {
         const int v = it % kVStages, b = it & 1;
         if (!wait(vfull(v), (it / kVStages) & 1) || !wait(wempty(b), ((it >> 1) & 1) ^ 1)) break;
@@ -329,57 +340,58 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     const int quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const bool live = row < valid;
-    const int token = live ? (int)((row0 + row) / p.group) : 0, qhead = head * p.group + (live ? (int)((row0 + row) % p.group) : 0);
+    const int token = live ? token0 + (head0 + row) / p.group : 0, qhead = head * p.group + (live ? (head0 + row) % p.group : 0);
     const int pos = live ? r.len - r.n + token : -1;
-    float qf;
     {
-      const uint4* qp = reinterpret_cast<const uint4*>(p.q + (int64_t)(r.r0 + token) * p.ld_q + (int64_t)qhead * D);
-      float amax = 0.0f;
-      bool bad = false;
-#pragma unroll 4
-      for (int c = 0; c < D / 8; ++c) {
-        const uint4 w = live ? __ldg(qp + c) : make_uint4(0, 0, 0, 0);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a = fabsf(__uint_as_float(u[j] << 16)), b = fabsf(__uint_as_float(u[j] & 0xFFFF0000u));
-          bad |= !(a < INFINITY) || !(b < INFINITY);
-          amax = fmaxf(amax, fmaxf(a, b));
-        }
+      // D / 8 lanes to a row, 8 channels each, so that a warp reads whole rows
+      constexpr int LPR = D / 8, RPW = 32 / LPR;
+      const int c = lane % LPR;                                              // 16 bytes of bf16 = half a 16-byte unit of codes
+      const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+      const __nv_bfloat16* const mine = p.q + (int64_t)(r.r0 + token) * p.ld_q + (int64_t)qhead * D;   // rows behind the last one: the first row's
+      // The warp's rows come in through the space of its f16 value tiles (free until the first of them is made), and a short loop turns
+      // them: unrolled over registers the same work was 13 KB of code that every CTA fetched once, 7 us.
+      uint8_t* const raw = smem + (w_at - base) + quarter * 32 * (2 * D);
+#pragma unroll 1
+      for (int i = 0; i < 32; i += RPW) {
+        const int e = i + lane / LPR;
+        const unsigned long long from = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), e) + 16 * c;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(raw + e * (2 * D) + 16 * c)), "l"(from) : "memory");
       }
-      const uint32_t u = __float_as_uint(amax);
-      const int e = max(-119, (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0));
-      const float inv = p.scale < 0.0f ? -pow2i(-e) : pow2i(-e);
-      qf = bad ? __uint_as_float(0x7FC00000u) : fabsf(p.scale) * pow2i(e);   // a query with an infinity or a NaN: NaN throughout
-      uint8_t* const hi_row = smem + row * 128;
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
 #pragma unroll 2
-      for (int c = 0; c < D / 16; ++c) {                                     // 16 channels: one 16-byte unit of each term
-        uint32_t h4[4], l4[4];
+      for (int i = 0; i < 32; i += RPW) {
+        const int e0 = i + lane / LPR, rr = quarter * 32 + e0;
+        const uint4 w = *reinterpret_cast<const uint4*>(raw + e0 * (2 * D) + 16 * c);
+        const __nv_bfloat162* const q2 = reinterpret_cast<const __nv_bfloat162*>(&w);
+        // the largest of the row, a NaN if it holds one
+        __nv_bfloat162 top = __hmax2_nan(__hmax2_nan(__habs2(q2[0]), __habs2(q2[1])), __hmax2_nan(__habs2(q2[2]), __habs2(q2[3])));
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const uint4 w = live ? __ldg(qp + 2 * c + s) : make_uint4(0, 0, 0, 0);
-          const uint32_t uw[4] = {w.x, w.y, w.z, w.w};
-          uint16_t h2[4], l2[4];
+        for (int o = LPR / 2; o > 0; o >>= 1) top = __hmax2_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float amax = __bfloat162float(__hmax_nan(top.x, top.y));
+        const uint32_t u = __float_as_uint(amax);
+        const int e = max(-119, (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0));
+        const float inv = sign * pow2i(-e);
+        uint16_t h[4], l[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float x = __uint_as_float(uw[j] << 16) * inv, y = __uint_as_float(uw[j] & 0xFFFF0000u) * inv;
-            const __nv_fp8x2_storage_t hh = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
-            const float2 b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(hh, __NV_E4M3)));
-            h2[j] = hh;
-            l2[j] = __nv_cvt_float2_to_fp8x2(make_float2(x - b.x, y - b.y), __NV_SATFINITE, __NV_E4M3);
-          }
-          h4[2 * s] = pack16(h2[0], h2[1]); h4[2 * s + 1] = pack16(h2[2], h2[3]);
-          l4[2 * s] = pack16(l2[0], l2[1]); l4[2 * s + 1] = pack16(l2[2], l2[3]);
+        for (int j = 0; j < 4; ++j) {                                        // exact in f16 down to 2^-24
+          const float2 x = __bfloat1622float2(q2[j]);
+          split_f16(pack_f16(x.x * inv, x.y * inv), h[j], l[j]);
         }
         // rows of 128 bytes, 128-byte swizzle; 64 channels: both terms share a row
-        *reinterpret_cast<uint4*>(hi_row + ((c ^ (row & 7)) << 4)) = make_uint4(h4[0], h4[1], h4[2], h4[3]);
-        if (D == 128) *reinterpret_cast<uint4*>(hi_row + kRows * 128 + ((c ^ (row & 7)) << 4)) = make_uint4(l4[0], l4[1], l4[2], l4[3]);
-        else *reinterpret_cast<uint4*>(hi_row + (((c + 4) ^ (row & 7)) << 4)) = make_uint4(l4[0], l4[1], l4[2], l4[3]);
+        uint8_t* const qrow = smem + rr * 128;
+        const int unit16 = c >> 1, in16 = (c & 1) * 8;
+        *reinterpret_cast<uint2*>(qrow + ((unit16 ^ (rr & 7)) << 4) + in16) = make_uint2(pack16(h[0], h[1]), pack16(h[2], h[3]));
+        *reinterpret_cast<uint2*>(qrow + (D == 128 ? kRows * 128 + ((unit16 ^ (rr & 7)) << 4) : ((unit16 + 4) ^ (rr & 7)) << 4) + in16) =
+            make_uint2(pack16(l[0], l[1]), pack16(l[2], l[3]));
+        // a query with an infinity or a NaN: NaN throughout
+        if (c == 0) s_m[rr] = amax < INFINITY ? fabsf(p.scale) * pow2i(e) : __uint_as_float(0x7FC00000u);
       }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(qready);
     }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(qready);
+    const float qf = s_m[row];
 
     float m = -INFINITY, l = 0.0f;
     int R = kNone;
@@ -391,23 +403,29 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       __syncwarp();
       tc_fence_after();
       const Info d = s_info[it % kInfo];
+      const bool whole = (d.w[0] & d.w[1] & d.w[2] & d.w[3]) >> 31 && d.j0 + kTile <= key_end;   // every key is there
+      // and every row sees every key (tile edges, windows and tiles walked in parts are masked)
+      const bool clear = whole && d.w[0] & d.w[1] & d.w[2] & d.w[3] & kTaken && d.j0 + kTile - 1 <= first_pos && (p.window <= 0 || d.j0 > last_pos - p.window);
+      // Masking rewrites S in TMEM, 16 columns at a time in a loop that stays rolled: as straight code between the load and its use it ran
+      // once or twice per CTA and cost it 8 us each time in instruction fetches.
+      if (!clear) {
+        const int top = pos - d.j0, low = p.window > 0 ? top - p.window : -1;      // columns low < j <= top
+#pragma unroll 1
+        for (int c = 0; c < kTile; c += 16) {
+          uint32_t x[16];
+          tmem_ld16(tmem + b * kTile + c + lanes, x);
+          tmem_ld_wait();
+          const int t2 = (s_info[it % kInfo].w[c >> 4] & kTaken ? top : -1) - c, l2 = low - c;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) if (j > t2 || j <= l2) x[j] = 0xFF800000u;
+          tmem_st16(tmem + b * kTile + c + lanes, x);
+        }
+        tmem_st_wait();
+      }
       uint32_t sr[64];
       tmem_ld32(tmem + b * kTile + lanes, *reinterpret_cast<uint32_t(*)[32]>(&sr[0]));
       tmem_ld32(tmem + b * kTile + 32 + lanes, *reinterpret_cast<uint32_t(*)[32]>(&sr[32]));
       tmem_ld_wait();
-
-      const bool whole = (d.w[0] & d.w[1] & d.w[2] & d.w[3]) >> 31 && d.j0 + kTile <= key_end;   // every key is there
-      // and every row sees every key (tile edges, windows and tiles walked in parts take the masking pass first)
-      const bool clear = whole && d.w[0] & d.w[1] & d.w[2] & d.w[3] & kTaken && d.j0 + kTile - 1 <= first_pos && (p.window <= 0 || d.j0 > last_pos - p.window);
-      if (!clear) {
-        const int top = pos - d.j0, low = p.window > 0 ? top - p.window : -1;      // columns low < j <= top
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int t2 = d.w[g] & kTaken ? top : -1;
-#pragma unroll
-          for (int j = 16 * g; j < 16 * g + 16; ++j) sr[j] = j <= t2 && j > low ? sr[j] : 0xFF800000u;
-        }
-      }
       int lead = kNone;
       float fs[4], mt = -INFINITY;
 #pragma unroll
@@ -431,8 +449,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int lv = (int)(d.w[g] >> 8 & 0xFF) - 127;
-        const float add = (float)(8 + lv - R) - back;
-        const uint64_t f2 = dup(fs[g]), add2 = dup(add);
+        const uint64_t f2 = dup(fs[g]), add2 = dup((float)(8 + lv - R) - back);
         uint64_t sum = 0;
 #pragma unroll
         for (int j = 16 * g; j < 16 * g + 16; j += 2) {
@@ -450,7 +467,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       __syncwarp();
       tc_fence_after();
       if (it > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
           tmem_ld32(tmem_o + c + lanes, o);
@@ -473,7 +490,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     if (split == 1) {
       const int64_t orow = (int64_t)(r.r0 + token) * (t.n_kv_heads * p.group) + qhead;
       const float inv = l == 0.0f ? 0.0f : __frcp_rn(l), up = R == kNone ? 0.0f : pow2i(R - 8);
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
         tmem_ld32(tmem_o + c + lanes, o);
@@ -530,7 +547,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(smem + row * (D * 4) + ((u ^ (row & 7)) << 4), c));
         acc.x += fo * x.x; acc.y += fo * x.y; acc.z += fo * x.z; acc.w += fo * x.w;
       }
-      const int tk = (int)((row0 + row) / p.group), hd = head * p.group + (int)((row0 + row) % p.group);
+      const int tk = token0 + (head0 + row) / p.group, hd = head * p.group + (head0 + row) % p.group;
       const int64_t orow = (int64_t)(r.r0 + tk) * (t.n_kv_heads * p.group) + hd;
       const float inv = ll == 0.0f ? 0.0f : __frcp_rn(ll), up = rr == kNone ? 0.0f : pow2i(rr - 8);
       const __nv_bfloat162 y0 = __floats2bfloat162_rn(acc.x * inv * up, acc.y * inv * up), y1 = __floats2bfloat162_rn(acc.z * inv * up, acc.w * inv * up);
