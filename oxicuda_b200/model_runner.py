@@ -7,6 +7,12 @@ crates/oxicuda-infer/src/cache/kv_quant.rs) -> attention over the dequantized pa
 `rms_norm_quantize_fp8` -> gate|up FP8 GEMM -> `b2q_swiglu_quantize_rows_bf16` -> down FP8 GEMM; the logits come from an
 FP8 lm_head.  Attention itself is outside the quantized-linear path and is plain torch (softmax(QK^T/sqrt(d))V per
 sequence); everything with a `b2q_` entry point goes through the C ABI.
+
+`LlamaConfig(recipe="block128")` selects the block-scaled form of the same layer: weights with one scale per 128 x 128 block,
+activations with one per (token, 128 channels), a paged E4M3 cache with one scale per (page, kv head), and attention that
+reads those pages on the device for the whole ragged batch at once: `rms_norm_quantize_fp8_block128` -> q|k|v
+`gemm_fp8_block128` -> rotary embedding -> `PagedFp8KvCache.append` -> `PagedFp8KvCache.attend` -> block quantizer -> o
+projection -> norm -> gate|up -> `swiglu_quantize_fp8_block128` -> down projection.
 """
 from __future__ import annotations
 
@@ -18,8 +24,9 @@ import torch
 from . import _lib as L
 from ._lib import default_handle, ptr
 from .dist_infer import Fp8Linear
-from .kv_cache import rms_norm_quantize_fp8
-from .quant import Fp8Codec
+from .blas import gemm_fp8_block128
+from .kv_cache import PagedFp8KvCache, rms_norm_quantize_fp8, rms_norm_quantize_fp8_block128
+from .quant import Fp8Codec, quantize_fp8_blocks, swiglu_quantize_fp8_block128
 
 
 class EmptyBatch(L.B2qError):
@@ -73,6 +80,24 @@ class LlamaConfig:
     rope_theta: float = 10000.0
     eps: float = 1e-5
     kv_bits: int = 8
+    recipe: str = "per_token"     # or "block128": scales per block of 128, E4M3 pages with a scale per page and head
+
+    def validate(self) -> None:
+        if self.recipe not in ("per_token", "block128"):
+            raise L.InvalidConfig(L.ERR_INVALID_CONFIG, f"recipe must be per_token or block128, got {self.recipe!r}")
+        if self.recipe == "block128" and (self.n_heads * self.head_dim) % 128 != 0:
+            raise L.InvalidConfig(L.ERR_INVALID_CONFIG, f"block128: n_heads * head_dim must be a multiple of 128, got {self.n_heads * self.head_dim}")
+
+
+class Fp8Block128Linear:
+    """A linear layer held as E4M3 codes with one scale per 128 x 128 block; forward(x_codes, x_scales) -> [tokens x out]."""
+
+    def __init__(self, weight: torch.Tensor):
+        self.out_features, self.in_features = weight.shape
+        self.codes, self.scales = quantize_fp8_blocks(weight, 128)
+
+    def forward(self, x_codes: torch.Tensor, x_scales: torch.Tensor, out: torch.Tensor = None) -> torch.Tensor:
+        return gemm_fp8_block128(x_codes, self.codes, x_scales, self.scales, out=out)
 
 
 class _Layer:
@@ -80,12 +105,16 @@ class _Layer:
         def w(rows, cols):
             return torch.randn(rows, cols, device=dev, generator=gen) * (1.0 / math.sqrt(cols))
         qkv_rows = (cfg.n_heads + 2 * cfg.n_kv_heads) * cfg.head_dim
-        self.qkv = Fp8Linear(w(qkv_rows, cfg.hidden))
-        self.o = Fp8Linear(w(cfg.hidden, cfg.n_heads * cfg.head_dim))
-        self.gate_up = Fp8Linear(w(2 * cfg.ffn, cfg.hidden))
-        self.down = Fp8Linear(w(cfg.hidden, cfg.ffn))
+        linear = Fp8Block128Linear if cfg.recipe == "block128" else Fp8Linear
+        self.qkv = linear(w(qkv_rows, cfg.hidden))
+        self.o = linear(w(cfg.hidden, cfg.n_heads * cfg.head_dim))
+        self.gate_up = linear(w(2 * cfg.ffn, cfg.hidden))
+        self.down = linear(w(cfg.hidden, cfg.ffn))
         self.g_attn = (1.0 + 0.05 * torch.randn(cfg.hidden, device=dev, generator=gen)).to(torch.bfloat16)
         self.g_mlp = (1.0 + 0.05 * torch.randn(cfg.hidden, device=dev, generator=gen)).to(torch.bfloat16)
+        if cfg.recipe == "block128":
+            self.cache = PagedFp8KvCache.empty(cfg.num_blocks, cfg.block_size, cfg.n_kv_heads, cfg.head_dim, dev)
+            return
         pages = cfg.num_blocks * cfg.block_size
         # paged KV cache: codes per (page slot, kv head, channel), one (scale, zero point) per (page slot, kv head)
         self.k_codes = torch.zeros(pages, cfg.n_kv_heads, cfg.head_dim, dtype=torch.uint8, device=dev)
@@ -98,12 +127,14 @@ class QuantizedLlamaRunner:
     """ModelRunner over random-init weights of the given shape (there are no checkpoints to load here)."""
 
     def __init__(self, cfg: LlamaConfig, device, seed: int = 0):
+        cfg.validate()
         self.cfg, self.dev = cfg, device
         gen = torch.Generator(device=device).manual_seed(seed)
         self.embed = (torch.randn(cfg.vocab_size, cfg.hidden, device=device, generator=gen) * 0.5).to(torch.bfloat16)
         self.layers = [_Layer(cfg, gen, device) for _ in range(cfg.n_layers)]
         self.g_final = (1.0 + 0.05 * torch.randn(cfg.hidden, device=device, generator=gen)).to(torch.bfloat16)
-        self.lm_head = Fp8Linear(torch.randn(cfg.vocab_size, cfg.hidden, device=device, generator=gen) * (1.0 / math.sqrt(cfg.hidden)))
+        head = torch.randn(cfg.vocab_size, cfg.hidden, device=device, generator=gen) * (1.0 / math.sqrt(cfg.hidden))
+        self.lm_head = Fp8Block128Linear(head) if cfg.recipe == "block128" else Fp8Linear(head)
         self.codec = Fp8Codec.e4m3("rne")
         self.trace = None          # a list here collects every stage's tensors per layer (tests check each stage on its own inputs)
         half = cfg.head_dim // 2
@@ -170,6 +201,8 @@ class QuantizedLlamaRunner:
     # ---- the forward pass over `tokens` rows; seqs = [(row_start, row_end, first_position, block_table)] ----------
     def _forward(self, token_ids: torch.Tensor, positions: torch.Tensor, seqs) -> torch.Tensor:
         cfg = self.cfg
+        if cfg.recipe == "block128":
+            return self._forward_block128(token_ids, positions, seqs)
         tokens = token_ids.numel()
         delta = self.embed[token_ids.long()].contiguous()                      # what the next norm adds to the residual
         res = torch.zeros(tokens, cfg.hidden, dtype=torch.bfloat16, device=self.dev)
@@ -204,6 +237,41 @@ class QuantizedLlamaRunner:
                                        mlp_out=delta))
         xc, xs = rms_norm_quantize_fp8(delta, self.g_final, cfg.eps, residual=res)
         return xc, xs
+
+    def _forward_block128(self, token_ids: torch.Tensor, positions: torch.Tensor, seqs):
+        cfg = self.cfg
+        tokens, nq, nkv, d = token_ids.numel(), cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
+        delta = self.embed[token_ids.long()].contiguous()
+        res = torch.zeros(tokens, cfg.hidden, dtype=torch.bfloat16, device=self.dev)
+        # the batch as the cache reads it: one upload each, nothing is read back
+        for r0, r1, p0, table in seqs:
+            if -(-(p0 + r1 - r0) // cfg.block_size) > len(table):
+                raise L.DimensionMismatch(L.ERR_DIMENSION_MISMATCH, f"expected {-(-(p0 + r1 - r0) // cfg.block_size)} KV blocks, got {len(table)}")
+            if any(not 0 <= b < cfg.num_blocks for b in table):
+                raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, f"block table {list(table)} names a block outside [0, {cfg.num_blocks})")
+        width = max(1, max(len(t) for _, _, _, t in seqs))
+        lens = torch.tensor([p0 + r1 - r0 for r0, r1, p0, _ in seqs], dtype=torch.int32, device=self.dev)
+        tables = torch.tensor([list(t) + [-1] * (width - len(t)) for _, _, _, t in seqs], dtype=torch.int32, device=self.dev)
+        single = all(r1 - r0 == 1 for r0, r1, _, _ in seqs)
+        starts = None if single else torch.tensor([r0 for r0, _, _, _ in seqs] + [seqs[-1][1]], dtype=torch.int32, device=self.dev)
+        for layer in self.layers:
+            x_in = delta
+            xc, xs = rms_norm_quantize_fp8_block128(delta, layer.g_attn, cfg.eps, residual=res)
+            res_attn = res.clone() if self.trace is not None else None
+            qkv = layer.qkv.forward(xc, xs)                                    # bf16 [tokens, (nq + 2 nkv) d]
+            q = self._rope(qkv[:, : nq * d].reshape(tokens, nq, d), positions)
+            k = self._rope(qkv[:, nq * d: (nq + nkv) * d].reshape(tokens, nkv, d), positions)
+            layer.cache.append(k, qkv[:, (nq + nkv) * d:].view(tokens, nkv, d), lens, tables, q_starts=starts)
+            attn = layer.cache.attend(q, lens, tables, q_starts=starts)
+            ac, as_ = quantize_fp8_blocks(attn.view(tokens, nq * d), 1)
+            delta = o_out = layer.o.forward(ac, as_)
+            xc, xs = rms_norm_quantize_fp8_block128(delta, layer.g_mlp, cfg.eps, residual=res)
+            gu = layer.gate_up.forward(xc, xs)                                 # gate | up
+            hc, hs = swiglu_quantize_fp8_block128(gu[:, : cfg.ffn], gu[:, cfg.ffn:])
+            delta = layer.down.forward(hc, hs)
+            if self.trace is not None:
+                self.trace.append(dict(x_in=x_in, res_attn=res_attn, qkv=qkv, attn=attn.clone(), o_out=o_out, res_mlp=res.clone(), gu=gu, mlp_out=delta))
+        return rms_norm_quantize_fp8_block128(delta, self.g_final, cfg.eps, residual=res)
 
     def _logits(self, xc: torch.Tensor, xs: torch.Tensor, rows) -> list:
         idx = torch.tensor(rows, device=self.dev, dtype=torch.long)

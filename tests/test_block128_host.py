@@ -107,3 +107,13 @@ def test_null_handle_is_refused_by_the_block128_entry_points(libb2q):
     assert libb2q.b2q_swiglu_quantize_fp8_block128_bf16(None, None, None, 1, 1, 1, 0, 1, None, None) == 8
     assert libb2q.b2q_kv8_append_bf16(None, None, None, 64, 64, 1, None, None, None, 1, 1, 1, 16, 1, 64, None, None, None, None) == 8
     assert libb2q.b2q_kv8_attention_bf16(None, None, 64, 1, 1, None, None, None, 1, 1, 1, 16, 1, 64, None, None, None, None, 1.0, 0, None, None) == 8
+
+
+def test_runner_recipe_is_validated(libb2q):
+    from oxicuda_b200 import _lib
+    from oxicuda_b200.model_runner import LlamaConfig
+    LlamaConfig().validate()
+    LlamaConfig(recipe="block128").validate()
+    for bad in (LlamaConfig(recipe="per_block"), LlamaConfig(recipe="block128", n_heads=3, n_kv_heads=1)):
+        with pytest.raises(_lib.InvalidConfig):
+            bad.validate()
