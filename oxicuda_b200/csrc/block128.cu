@@ -16,14 +16,28 @@ namespace {
 
 constexpr float kMinScale = 1.17549435e-38f;   // 2^-126: its reciprocal is finite
 
-__device__ __forceinline__ void unpack8(const uint4 q, float (&v)[8]) {
+// Two neighbouring elements travel in one 64-bit register (low half first): the multiply-adds of sm_100a take both at once.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) { return (uint64_t)__float_as_uint(hi) << 32 | __float_as_uint(lo); }
+__device__ __forceinline__ float lo(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) { uint64_t r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y)); return r; }
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y)); return r; }
+__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t x, uint64_t y) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(x), "l"(y)); }
+__device__ __forceinline__ void unpack8(const uint4 q, uint64_t (&v)[4]) {
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) { v[2 * j] = __uint_as_float(w[j] << 16); v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u); }
+  for (int j = 0; j < 4; ++j) v[j] = (uint64_t)(w[j] & 0xFFFF0000u) << 32 | (w[j] << 16);
 }
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
-  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&p);
+}
+// bf16(a + b) of two pairs: a sum of two bf16 rounded once.  Rounding it to f32 first gives the same: where f32 rounds at all, the operands
+// are more than 2^16 apart and the sum is no tie of bf16.
+__device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 __device__ __forceinline__ float block_scale(float amax, float max_val) {
   return amax > 0.0f ? fmaxf(__fdiv_rn(amax, max_val), kMinScale) : 1.0f;
@@ -34,18 +48,24 @@ __device__ __forceinline__ uint32_t encode1(float v, float inv_scale, int fmt, i
   q = q < -F.max_val ? -F.max_val : (q > F.max_val ? F.max_val : q);
   return fp8_encode_ref_dev(q, F);
 }
-__device__ __forceinline__ uint2 encode8(const float (&v)[8], float inv_scale, int fmt, int rounding, const Fp8Fmt& F) {
-  if (rounding == B2Q_ROUND_RNE) {             // the conversion saturates to +-max_val by itself
+// What the kernels are compiled for: E4M3 to nearest even (the production form), or anything else (format and rounding at run time).
+enum Mode { kE4m3Rne, kAny };
+template <int MODE>
+__device__ __forceinline__ uint2 encode8(const uint64_t (&v)[4], float inv_scale, int fmt, int rounding, const Fp8Fmt& F) {
+  if (MODE == kE4m3Rne) {                      // the conversion saturates to +-448 by itself
+    const uint64_t inv = pair(inv_scale, inv_scale);
     uint32_t p[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      p[j] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(v[2 * j], inv_scale), __fmul_rn(v[2 * j + 1], inv_scale)),
-                                                __NV_SATFINITE, fmt == B2Q_FP8_E4M3 ? __NV_E4M3 : __NV_E5M2);
+    for (int j = 0; j < 4; ++j) {
+      const uint64_t q = mul2(v[j], inv);
+      p[j] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo(q), hi(q)), __NV_SATFINITE, __NV_E4M3);
+    }
     return make_uint2(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410));
   }
   uint32_t w[2] = {0, 0};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) w[j >> 2] |= encode1(v[j], inv_scale, fmt, rounding, F) << (8 * (j & 3));
+  for (int j = 0; j < 4; ++j)
+    w[j >> 1] |= (encode1(lo(v[j]), inv_scale, fmt, rounding, F) | encode1(hi(v[j]), inv_scale, fmt, rounding, F) << 8) << (16 * (j & 1));
   return make_uint2(w[0], w[1]);
 }
 // max over the 16 lanes that hold one block of 128 columns
@@ -54,11 +74,24 @@ __device__ __forceinline__ float max16(float v) {
   for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-__device__ __forceinline__ float absmax8(const float (&v)[8]) {
+__device__ __forceinline__ float absmax8(const uint64_t (&v)[4]) {
   float a = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) a = fmaxf(a, fabsf(v[j]));
+  for (int j = 0; j < 4; ++j) a = fmaxf(a, fmaxf(fabsf(lo(v[j])), fabsf(hi(v[j]))));
   return a;
+}
+// The scales of the N blocks that a group of 16 lanes holds: lane k of the group makes the k'th (a division and a reciprocal are some
+// twenty instructions each), the others get its reciprocal.  `mine` is the scale that this lane made (k < N).
+template <int N>
+__device__ __forceinline__ void block_scales(const float (&amax)[N], float max_val, float& mine, float (&inv)[N]) {
+  const int lane = threadIdx.x & 31, sub = lane & 15;
+  float a = amax[0];
+#pragma unroll
+  for (int k = 1; k < N; ++k) a = sub == k ? amax[k] : a;
+  mine = block_scale(a, max_val);
+  const float r = __frcp_rn(mine);
+#pragma unroll
+  for (int k = 0; k < N; ++k) inv[k] = N == 1 ? r : __shfl_sync(0xffffffffu, r, (lane & 16) | k);
 }
 __device__ __forceinline__ float block_sum(float v, float* sh) {
 #pragma unroll
@@ -81,7 +114,7 @@ struct NormArgs {
 
 // One CTA per row; thread t keeps chunks t, t + blockDim, ... (8 elements each, NCH at most) of the row in registers.
 // blockDim is a multiple of 32, so 16 neighbouring lanes always hold the 16 chunks of one block of 128 columns.
-template <int NCH>
+template <int NCH, int MODE>
 __global__ void __launch_bounds__(1024) rms_norm_block128_kernel(const NormArgs p) {
   b2q_pdl_entry();
   __shared__ float sh[32];
@@ -90,54 +123,60 @@ __global__ void __launch_bounds__(1024) rms_norm_block128_kernel(const NormArgs 
   const uint4* xr = reinterpret_cast<const uint4*>(p.x + r * p.cols);
   uint4* rr = p.residual ? reinterpret_cast<uint4*>(p.residual + r * p.cols) : nullptr;
   const uint4* gr = reinterpret_cast<const uint4*>(p.gamma);
-  float v[NCH][8];
+  uint4 xq[NCH];
   {
-    uint4 xq[NCH], rq[NCH];
+    uint4 rq[NCH];
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {                        // all loads of the row before the first use
       const int c = (int)threadIdx.x + k * (int)blockDim.x;
       xq[k] = c < chunks ? __ldcs(xr + c) : make_uint4(0, 0, 0, 0);
       if (rr) rq[k] = c < chunks ? __ldcs(rr + c) : make_uint4(0, 0, 0, 0);
     }
+    if (rr) {
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-      unpack8(xq[k], v[k]);
-      if (rr) {
-        float res[8];
-        unpack8(rq[k], res);
-        uint4 w;                                           // the norm is taken of the sum as it is stored
-        w.x = bf16_pair(__fadd_rn(res[0], v[k][0]), __fadd_rn(res[1], v[k][1]));
-        w.y = bf16_pair(__fadd_rn(res[2], v[k][2]), __fadd_rn(res[3], v[k][3]));
-        w.z = bf16_pair(__fadd_rn(res[4], v[k][4]), __fadd_rn(res[5], v[k][5]));
-        w.w = bf16_pair(__fadd_rn(res[6], v[k][6]), __fadd_rn(res[7], v[k][7]));
+      for (int k = 0; k < NCH; ++k) {                      // the norm is taken of the sum as it is stored
         const int c = (int)threadIdx.x + k * (int)blockDim.x;
-        if (c < chunks) rr[c] = w;
-        unpack8(w, v[k]);
+        xq[k] = make_uint4(add_bf16x2(rq[k].x, xq[k].x), add_bf16x2(rq[k].y, xq[k].y), add_bf16x2(rq[k].z, xq[k].z), add_bf16x2(rq[k].w, xq[k].w));
+        if (c < chunks) rr[c] = xq[k];
       }
     }
   }
-  float ss = 0.0f;
+  uint64_t s2 = 0;
 #pragma unroll
-  for (int k = 0; k < NCH; ++k)
+  for (int k = 0; k < NCH; ++k) {
+    uint64_t v[4];
+    unpack8(xq[k], v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(v[k][j], v[k][j], ss);
-  ss = block_sum(ss, sh);
+    for (int j = 0; j < 4; ++j) fma2(s2, v[j], v[j]);
+  }
+  const float ss = block_sum(lo(s2) + hi(s2), sh);
   const float inv_rms = __frcp_rn(sqrtf(__fadd_rn(__fdiv_rn(ss, (float)p.cols), p.eps)));
+  const uint64_t inv2 = pair(inv_rms, inv_rms);
   const Fp8Fmt F = fp8_fmt(p.fmt);
   uint2* cr = reinterpret_cast<uint2*>(p.codes + r * p.cols);
   uint4* yr = p.y ? reinterpret_cast<uint4*>(p.y + r * p.cols) : nullptr;
+  uint64_t v[NCH][4];
+  float amax[NCH], inv[NCH], mine;
 #pragma unroll
   for (int k = 0; k < NCH; ++k) {
     const int c = (int)threadIdx.x + k * (int)blockDim.x;
-    float g[8];
+    uint64_t g[4];
     unpack8(c < chunks ? __ldg(gr + c) : make_uint4(0, 0, 0, 0), g);
+    unpack8(xq[k], v[k]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[k][j] = c < chunks ? __fmul_rn(__fmul_rn(v[k][j], inv_rms), g[j]) : 0.0f;
-    const float scale = block_scale(max16(absmax8(v[k])), F.max_val);
+    for (int j = 0; j < 4; ++j) v[k][j] = mul2(mul2(v[k][j], inv2), g[j]);
+    amax[k] = max16(c < chunks ? absmax8(v[k]) : 0.0f);    // (0 * inf behind the row's end would be a NaN, which the maximum passes over)
+  }
+  block_scales<NCH>(amax, F.max_val, mine, inv);
+#pragma unroll
+  for (int k = 0; k < NCH; ++k) {
+    const int c = (int)threadIdx.x + k * (int)blockDim.x;
+    if ((threadIdx.x & 15) == k && (c & ~15) < chunks) p.scales[r * nb + (c >> 4)] = mine;
     if (c < chunks) {
-      cr[c] = encode8(v[k], __frcp_rn(scale), p.fmt, p.rounding, F);
-      if ((c & 15) == 0) p.scales[r * nb + (c >> 4)] = scale;
-      if (yr) yr[c] = make_uint4(bf16_pair(v[k][0], v[k][1]), bf16_pair(v[k][2], v[k][3]), bf16_pair(v[k][4], v[k][5]), bf16_pair(v[k][6], v[k][7]));
+      cr[c] = encode8<MODE>(v[k], inv[k], p.fmt, p.rounding, F);
+      if (yr)
+        yr[c] = make_uint4(bf16_pair(lo(v[k][0]), hi(v[k][0])), bf16_pair(lo(v[k][1]), hi(v[k][1])), bf16_pair(lo(v[k][2]), hi(v[k][2])),
+                           bf16_pair(lo(v[k][3]), hi(v[k][3])));
     }
   }
 }
@@ -186,43 +225,84 @@ __global__ void __launch_bounds__(256) rms_norm_block128_generic_kernel(const No
   }
 }
 
-// silu(g) = g / (1 + e^-g) with e^-|g|, which cannot overflow: g e^g / (1 + e^g) for negative g.  silu(g) before u: g * u may
-// overflow where silu(g) is next to 0.
-__device__ __forceinline__ float swiglu(float g, float u) {
+// silu(g) = g / (1 + e^-g), two at a time, by the hardware's exponential and reciprocal (2^-22 and 1 ulp; 1 + e^-g is never below 1, so
+// neither needs the handling of subnormals that makes their exact forms several instructions each: with those the kernel was
+// instruction-bound, 84 us for 2047 x 28672).  Where e^-g passes the f32 range the result is 0 instead of a number below 2^-121: see tiny().
+// silu(g) before u: g * u may overflow where silu(g) is next to 0.
+__device__ __forceinline__ uint64_t silu2(uint64_t g) {
+  const uint64_t t = mul2(g, pair(-1.4426950408889634f, -1.4426950408889634f));
+  float ea, eb, ra, rb;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(ea) : "f"(lo(t)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(eb) : "f"(hi(t)));
+  const uint64_t d = add2(pair(ea, eb), pair(1.0f, 1.0f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(ra) : "f"(lo(d)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rb) : "f"(hi(d)));
+  return mul2(g, pair(ra, rb));
+}
+// A block this small may be made of results that silu2 has rounded to 0: it is made again by silu_exact, g e^g / (1 + e^g) for negative g.
+__device__ __forceinline__ bool tiny(float amax) { return amax < 7.9e-31f; }   // 2^-100
+__device__ __forceinline__ float silu_exact(float g) {
   const float e = exp2f(-1.4426950408889634f * fabsf(g));
-  return g * (g < 0.0f ? e : 1.0f) * __frcp_rn(1.0f + e) * u;
+  return g * (g < 0.0f ? e : 1.0f) * __frcp_rn(1.0f + e);
 }
 
 struct SwigluArgs {
   const __nv_bfloat16* gate; const __nv_bfloat16* up; int64_t rows, cols, ld; int fmt, rounding;
   float* scales; uint8_t* codes;
+  uint32_t per_row, magic;                       // blocks of a row, floor((2^32 - 1) / per_row)
 };
 
-// 16 lanes per block of 128 columns, a warp two blocks; the blocks of all rows are one flat index space.
+// 16 lanes per block of 128 columns, a warp two blocks; the blocks of all rows are one flat index space (below 2^31, so that its
+// division by the blocks of a row is a multiplication), two steps of it in flight per thread.
+template <int MODE>
 __global__ void __launch_bounds__(256) swiglu_block128_kernel(const SwigluArgs p) {
   b2q_pdl_entry();
-  const int64_t nb = (p.cols + 127) >> 7, total = p.rows * nb;
+  const uint32_t total = (uint32_t)p.rows * p.per_row, step = gridDim.x * 16;
   const int sub = threadIdx.x & 15;
   const Fp8Fmt F = fp8_fmt(p.fmt);
-  const int64_t step = (int64_t)gridDim.x * 16;
-  for (int64_t b0 = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); b0 - (int64_t)((threadIdx.x >> 4) & 1) < total; b0 += step) {   // whole warps leave together
-    const int64_t r = b0 / nb, b = b0 - r * nb, c = b * 128 + sub * 8;
-    const bool live = b0 < total && c < p.cols;
-    float h[8];
-    if (live) {
-      float g[8], u[8];
-      unpack8(__ldcs(reinterpret_cast<const uint4*>(p.gate + r * p.ld + c)), g);
-      unpack8(__ldcs(reinterpret_cast<const uint4*>(p.up + r * p.ld + c)), u);
+  for (uint32_t first = blockIdx.x * 16; first < total; first += 2 * step) {       // the whole CTA leaves together
+    uint4 gq[2], uq[2];
+    uint32_t at[2], row[2], col[2];
+    bool live[2];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[j] = swiglu(g[j], u[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) h[j] = 0.0f;
+    for (int k = 0; k < 2; ++k) {
+      at[k] = first + k * step + (threadIdx.x >> 4);
+      row[k] = __umulhi(at[k], p.magic);
+      uint32_t b = at[k] - row[k] * p.per_row;
+      if (b >= p.per_row) { b -= p.per_row; ++row[k]; }                            // the product is at most one short
+      col[k] = b * 128 + sub * 8;
+      live[k] = at[k] < total && col[k] < p.cols;
+      gq[k] = uq[k] = make_uint4(0, 0, 0, 0);
+      if (live[k]) {
+        gq[k] = __ldcs(reinterpret_cast<const uint4*>(p.gate + row[k] * p.ld + col[k]));
+        uq[k] = __ldcs(reinterpret_cast<const uint4*>(p.up + row[k] * p.ld + col[k]));
+      }
     }
-    const float scale = block_scale(max16(absmax8(h)), F.max_val);
-    if (live) {
-      *reinterpret_cast<uint2*>(p.codes + r * p.cols + c) = encode8(h, __frcp_rn(scale), p.fmt, p.rounding, F);
-      if (sub == 0) p.scales[b0] = scale;
+    uint64_t h[2][4];
+    float amax[2], inv[2], mine;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint64_t g[4], u[4];
+      unpack8(gq[k], g);
+      unpack8(uq[k], u);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[k][j] = mul2(silu2(g[j]), u[j]);               // zeros where nothing was loaded
+      amax[k] = max16(absmax8(h[k]));
+      if (__any_sync(0xffffffffu, tiny(amax[k]))) {                                // (a block of zeros comes this way too)
+        if (live[k] && tiny(amax[k])) {
+          const __nv_bfloat16 *gp = p.gate + row[k] * p.ld + col[k], *up = p.up + row[k] * p.ld + col[k];   // read again: nothing is held for this path
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            h[k][j] = pair(silu_exact(__bfloat162float(gp[2 * j])) * __bfloat162float(up[2 * j]), silu_exact(__bfloat162float(gp[2 * j + 1])) * __bfloat162float(up[2 * j + 1]));
+        }
+        amax[k] = max16(absmax8(h[k]));
+      }
+    }
+    block_scales<2>(amax, F.max_val, mine, inv);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (sub == k && at[k] < total) p.scales[at[k]] = mine;
+      if (live[k]) *reinterpret_cast<uint2*>(p.codes + row[k] * p.cols + col[k]) = encode8<MODE>(h[k], inv[k], p.fmt, p.rounding, F);
     }
   }
 }
@@ -239,7 +319,7 @@ __global__ void __launch_bounds__(256) swiglu_block128_generic_kernel(const Swig
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t c = b * 128 + j * 32 + lane;
-      h[j] = c < p.cols ? swiglu(__bfloat162float(p.gate[r * p.ld + c]), __bfloat162float(p.up[r * p.ld + c])) : 0.0f;
+      h[j] = c < p.cols ? silu_exact(__bfloat162float(p.gate[r * p.ld + c])) * __bfloat162float(p.up[r * p.ld + c]) : 0.0f;
       amax = fmaxf(amax, fabsf(h[j]));
     }
     const float scale = block_scale(warp_max(amax), F.max_val), inv = __frcp_rn(scale);
@@ -273,9 +353,11 @@ extern "C" int32_t b2q_rms_norm_quantize_fp8_block128_bf16(b2q_handle h, const v
     int nch = chunks <= 1024 ? 1 : (chunks <= 2048 ? 2 : 4);
     if (rows >= 2 * (int64_t)h->sm_count && chunks > 128) nch = chunks <= 256 ? 2 : 4;
     const dim3 block((unsigned)(ceil_div64(ceil_div64(chunks, nch), 32) * 32));
-    if (nch == 1) B2Q_CUDA(h, b2q_pdl_launch(pdl, rms_norm_block128_kernel<1>, grid, block, 0, h->stream, p));
-    else if (nch == 2) B2Q_CUDA(h, b2q_pdl_launch(pdl, rms_norm_block128_kernel<2>, grid, block, 0, h->stream, p));
-    else B2Q_CUDA(h, b2q_pdl_launch(pdl, rms_norm_block128_kernel<4>, grid, block, 0, h->stream, p));
+    const bool main = fmt == B2Q_FP8_E4M3 && rounding == B2Q_ROUND_RNE;
+    auto kernel = nch == 1 ? (main ? rms_norm_block128_kernel<1, kE4m3Rne> : rms_norm_block128_kernel<1, kAny>)
+                : nch == 2 ? (main ? rms_norm_block128_kernel<2, kE4m3Rne> : rms_norm_block128_kernel<2, kAny>)
+                           : (main ? rms_norm_block128_kernel<4, kE4m3Rne> : rms_norm_block128_kernel<4, kAny>);
+    B2Q_CUDA(h, b2q_pdl_launch(pdl, kernel, grid, block, 0, h->stream, p));
     return B2Q_OK;
   }
   B2Q_CUDA(h, b2q_pdl_launch(pdl, rms_norm_block128_generic_kernel, grid, dim3(256), 0, h->stream, p));
@@ -288,12 +370,15 @@ extern "C" int32_t b2q_swiglu_quantize_fp8_block128_bf16(b2q_handle h, const voi
   if (rows <= 0 || cols <= 0) B2Q_FAIL(h, B2Q_ERR_EMPTY_INPUT, "swiglu_quantize_fp8_block128: empty input");
   if (!gate || !up || !scales || !codes || ld < cols) B2Q_FAIL(h, B2Q_ERR_INVALID_ARGUMENT, "swiglu_quantize_fp8_block128: null pointer, or ld < cols");
   if (fmt < 0 || fmt > 1 || rounding < 0 || rounding > 1) B2Q_FAIL(h, B2Q_ERR_INVALID_ARGUMENT, "swiglu_quantize_fp8_block128: bad format/rounding");
-  SwigluArgs p{static_cast<const __nv_bfloat16*>(gate), static_cast<const __nv_bfloat16*>(up), rows, cols, ld, fmt, rounding, scales, codes};
-  const int64_t total = rows * ceil_div64(cols, 128);
-  const bool vec = cols % 8 == 0 && ld % 8 == 0 && ((reinterpret_cast<uintptr_t>(gate) | reinterpret_cast<uintptr_t>(up)) & 15) == 0 &&
+  const int64_t per_row = ceil_div64(cols, 128), total = rows * per_row;
+  SwigluArgs p{static_cast<const __nv_bfloat16*>(gate), static_cast<const __nv_bfloat16*>(up), rows, cols, ld, fmt, rounding, scales, codes,
+               (uint32_t)per_row, 0xFFFFFFFFu / (uint32_t)(per_row > 0xFFFFFFFFll ? 1 : per_row)};
+  const bool vec = total < (1ll << 31) && cols < (1ll << 31) && cols % 8 == 0 && ld % 8 == 0 && ((reinterpret_cast<uintptr_t>(gate) | reinterpret_cast<uintptr_t>(up)) & 15) == 0 &&
                    (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
-  const int64_t ctas = ceil_div64(total, vec ? 16 : 8), most = (int64_t)h->sm_count * 32;
+  const int64_t ctas = ceil_div64(total, vec ? 16 : 8), most = (int64_t)h->sm_count * (vec ? 24 : 32);
   const dim3 grid((unsigned)(ctas < most ? ctas : most));
-  B2Q_CUDA(h, b2q_pdl_launch(h->sw.chain_pdl != 0, vec ? swiglu_block128_kernel : swiglu_block128_generic_kernel, grid, dim3(256), 0, h->stream, p));
+  auto kernel = !vec ? swiglu_block128_generic_kernel
+                     : fmt == B2Q_FP8_E4M3 && rounding == B2Q_ROUND_RNE ? swiglu_block128_kernel<kE4m3Rne> : swiglu_block128_kernel<kAny>;
+  B2Q_CUDA(h, b2q_pdl_launch(h->sw.chain_pdl != 0, kernel, grid, dim3(256), 0, h->stream, p));
   return B2Q_OK;
 }

@@ -67,6 +67,7 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(const AppendArgs p) {
 
   float amax = 0.0f;
   bool bad = false;
+#pragma unroll 8
   for (int i = row; i < hi - lo; i += RPW) {
     const uint4 q = *reinterpret_cast<const uint4*>(x + (int64_t)i * p.ld[kv] + sub * 8);
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
@@ -105,6 +106,7 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(const AppendArgs p) {
     }
   }
   const float inv = pow2f(-e);
+#pragma unroll 8
   for (int i = row; i < hi - lo; i += RPW) {
     const uint4 q = *reinterpret_cast<const uint4*>(x + (int64_t)i * p.ld[kv] + sub * 8);
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
