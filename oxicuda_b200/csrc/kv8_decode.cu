@@ -25,6 +25,7 @@
 #include "kv8.cuh"
 #include "tc_common.cuh"
 #include <cooperative_groups.h>
+#include <stdlib.h>
 
 namespace cg = cooperative_groups;
 
@@ -45,7 +46,7 @@ constexpr int kNone = -1000;                     // R of a warp that has seen no
 constexpr int kSpan = 8;                         // value scales that share a product differ by at most 2^kSpan
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -97,6 +98,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   uint4* const s_info = reinterpret_cast<uint4*>(ring + G::kStages * G::kStage + 16 * G::kStages);   // [stage], one word per 16 keys
   float (*const s_o)[kRows][D] = reinterpret_cast<float (*)[kRows][D]>(ring);                       // [kWarps], when the ring is done with
   static_assert(kWarps * kRows * D * 4 <= G::kStages * G::kStage, "the join reuses the ring");
+  __shared__ int4 s_line[32];                    // the producer's next tiles: lines of their pages, scales
+  __shared__ uint4 s_words[32];
   __shared__ int s_abort;
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
   __shared__ int s_r[kWarps];
@@ -105,7 +108,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 
   if (threadIdx.x == 0) {
     s_abort = 0;
-    for (int i = 0; i < G::kStages; ++i) { mbar_init(full_bar(i), 1); mbar_init(empty_bar(i), 2); }
+    for (int i = 0; i < G::kStages; ++i) { mbar_init(full_bar(i), 2); mbar_init(empty_bar(i), 2); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
@@ -125,14 +128,14 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     f = make_int2(unit / per, unit % per);
   } else {
     if (unit == 0 && tell) for (int b = lane; b < t.seqs; b += 32) rows_of(t, b, true);
-    f = find_unit(t.seqs, unit, [&](int b) { return (int)(((int64_t)rows_of(t, b, false).n * p.group + kRows - 1) / kRows); });
+    f = find_unit(t.seqs, unit, [&](int b) { return (rows_of(t, b, false).n * p.group + kRows - 1) / kRows; });
     if (f.x < 0) return;                          // the whole cluster leaves: every CTA of it has the same unit
   }
   const Rows r = rows_of(t, f.x, tell && t.q_starts == nullptr && lane == 0);
-  const int64_t rows = (int64_t)r.n * p.group, row0 = (int64_t)f.y * kRows;
-  const int valid = (int)min((int64_t)kRows, rows - row0);            // <= 0: an impossible sequence, its rows stay as they are
-  if (valid <= 0) return;
-  const int first_pos = r.len - r.n + (int)(row0 / p.group), last_pos = r.len - r.n + (int)((row0 + valid - 1) / p.group);
+  const int row0 = f.y * kRows, valid = min(kRows, r.n * p.group - row0);   // rows of all sequences fit 31 bits; <= 0: an impossible sequence
+  if (valid <= 0) return;                         // its rows stay as they are
+  const int token0 = row0 / p.group, head0 = row0 - token0 * p.group;       // of the first row, within the sequence and the group
+  const int first_pos = r.len - r.n + token0, last_pos = first_pos + (head0 + valid - 1) / p.group;
   const int key_end = last_pos + 1;
   const int key_begin = p.window > 0 ? max(0, first_pos - p.window + 1) & ~(kTile - 1) : 0;
 
@@ -157,60 +160,74 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const int subs = t.page_shift >= 6 ? 1 : 64 >> t.page_shift, rows_each = kTile / subs;   // pages that a tile spans, their keys
     int pg[4];
     uint32_t info[4];
-    auto fetch = [&](int i0) {
+    auto pages = [&](int i0) {
       const int j0 = key_begin + kTile * (part + split * (i0 + lane));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        pg[e] = -1; info[e] = 0;
         const int j = j0 + rows_each * e;
-        if (e < subs && i0 + lane < mine && j < key_end) {
-          pg[e] = page_of(t, f.x, j >> t.page_shift, head == 0);
-          if (pg[e] >= 0)
-            info[e] = 0x80000000u | (uint32_t)p.ks[(int64_t)pg[e] * t.n_kv_heads + head] | ((uint32_t)p.vs[(int64_t)pg[e] * t.n_kv_heads + head] << 8);
-        }
+        pg[e] = e < subs && i0 + lane < mine && j < key_end ? page_of(t, f.x, j >> t.page_shift, head == 0) : -1;
       }
     };
-    bool ok = true;
-    fetch(0);
-    for (int i0 = 0; i0 < mine && ok; i0 += 32) {
-      int cp[4];
-      uint32_t ci[4];
+    auto scales = [&] {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { cp[e] = pg[e]; ci[e] = info[e]; }
-      if (i0 + 32 < mine) fetch(i0 + 32);
-      const int n = min(32, mine - i0);
-      for (int i = 0; i < n; ++i) {
-        const int it = i0 + i, st = it % G::kStages, j = key_begin + kTile * (part + split * it);
-        int p4[4];
-        uint32_t f4[4];
+      for (int e = 0; e < 4; ++e)
+        info[e] = pg[e] < 0 ? 0u : 0x80000000u | (uint32_t)p.ks[(int64_t)pg[e] * t.n_kv_heads + head] | ((uint32_t)p.vs[(int64_t)pg[e] * t.n_kv_heads + head] << 8);
+    };
+    // A lane leaves the lines of its tile's pages (the maps see lines of 128 bytes: one token of 128 channels, or two of 64; -1: no page) and
+    // the scales in shared memory; lane 0 alone issues, without a step of the other lanes in between.
+    auto leave = [&](int i0) {
+      const int in_page = (key_begin + kTile * (part + split * (i0 + lane))) & ((1 << t.page_shift) - 1);   // 0 but for pages of 128
+      int line[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (e >= subs) { p4[e] = -1; f4[e] = 0; continue; }
-          p4[e] = __shfl_sync(0xffffffffu, cp[e], i); f4[e] = __shfl_sync(0xffffffffu, ci[e], i);
-        }
-        if (lane == 0) {
-          ok = mbar_wait_bounded(empty_bar(st), ((it / G::kStages) & 1) ^ 1, abort_flag, kWaitLimitNs, 1);
-          if (ok) {
-            s_info[st] = subs == 1 ? make_uint4(f4[0], f4[0], f4[0], f4[0]) : subs == 2 ? make_uint4(f4[0], f4[0], f4[1], f4[1]) : make_uint4(f4[0], f4[1], f4[2], f4[3]);
-            const int in_page = j & ((1 << t.page_shift) - 1);        // 0 but for pages of 128
-            int there = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) there += p4[e] >= 0;
-            const uint32_t dk = base + st * G::kStage, dv = dk + G::kHalf;
-            mbar_expect_tx(full_bar(st), (uint32_t)(there * rows_each) * 2 * D);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (p4[e] < 0) continue;
-              // the maps see lines of 128 bytes: one token of 128 channels, or two of 64
-              const int line = (((p4[e] * t.n_kv_heads + head) << t.page_shift) + in_page) / (128 / D);
-              tma_load_2d(dk + e * rows_each * D, &map_k, full_bar(st), 0, line);
-              tma_load_2d(dv + e * rows_each * D, &map_v, full_bar(st), 0, line);
-            }
-          }
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) break;
+      for (int e = 0; e < 4; ++e) line[e] = pg[e] < 0 ? -1 : (((pg[e] * t.n_kv_heads + head) << t.page_shift) + in_page) / (128 / D);
+      s_line[lane] = make_int4(line[0], line[1], line[2], line[3]);
+    };
+    auto words = [&] {
+      return subs == 1 ? make_uint4(info[0], info[0], info[0], info[0]) : subs == 2 ? make_uint4(info[0], info[0], info[1], info[1])
+                                                                                     : make_uint4(info[0], info[1], info[2], info[3]);
+    };
+    const uint32_t bytes = (uint32_t)rows_each * D;
+    auto copy = [&](int st, const int4 ln) {
+      const uint32_t dk = base + st * G::kStage, dv = dk + G::kHalf, bar = full_bar(st);
+      const int there = (ln.x >= 0) + (ln.y >= 0) + (ln.z >= 0) + (ln.w >= 0);
+      mbar_expect_tx(bar, there * 2 * bytes);
+      if (ln.x >= 0) { tma_load_2d(dk, &map_k, bar, 0, ln.x); tma_load_2d(dv, &map_v, bar, 0, ln.x); }
+      if (subs > 1) {
+        if (ln.y >= 0) { tma_load_2d(dk + bytes, &map_k, bar, 0, ln.y); tma_load_2d(dv + bytes, &map_v, bar, 0, ln.y); }
+        if (ln.z >= 0) { tma_load_2d(dk + 2 * bytes, &map_k, bar, 0, ln.z); tma_load_2d(dv + 2 * bytes, &map_v, bar, 0, ln.z); }
+        if (ln.w >= 0) { tma_load_2d(dk + 3 * bytes, &map_k, bar, 0, ln.w); tma_load_2d(dv + 3 * bytes, &map_v, bar, 0, ln.w); }
       }
+    };
+    // the first copies go out before the scales are known, and the scales arrive while they fly
+    bool ok = true;
+    const int lead_in = min(mine, G::kStages);
+    pages(0);
+    leave(0);
+    __syncwarp();
+    if (lane == 0) for (int i = 0; i < lead_in; ++i) copy(i, s_line[i]);
+    scales();
+    if (lane < lead_in) {
+      s_info[lane] = words();
+      mbar_arrive(full_bar(lane));                // the second of a stage's two arrivals
+    }
+    for (int i0 = 0; i0 < mine && ok; i0 += 32) {
+      s_words[lane] = words();
+      __syncwarp();
+      if (i0 + 32 < mine) { pages(i0 + 32); scales(); }                // in flight while lane 0 issues
+      if (lane == 0) {
+        const int n = min(32, mine - i0);
+        for (int i = i0 ? 0 : lead_in; i < n; ++i) {
+          const int st = (i0 + i) % G::kStages;
+          const int4 ln = s_line[i];
+          const uint4 w = s_words[i];
+          if (!mbar_wait_bounded(empty_bar(st), (((i0 + i) / G::kStages) & 1) ^ 1, abort_flag, kWaitLimitNs, 1)) { ok = false; break; }
+          copy(st, ln);
+          s_info[st] = w;
+          mbar_arrive(full_bar(st));
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      leave(i0 + 32);
     }
     if (!ok && lane == 0) {                      // give copies in flight time to land before shared memory is released
       const uint64_t t0 = globaltimer_ns();
@@ -225,7 +242,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     for (int x = 0; x < RB; ++x) {
       const int row = 8 * x + lr;
       const bool live = row < valid;
-      const int token = live ? (int)((row0 + row) / p.group) : 0, g = live ? (int)((row0 + row) % p.group) : 0;
+      const int token = live ? token0 + (head0 + row) / p.group : token0, g = live ? (head0 + row) % p.group : 0;
       const __nv_bfloat16* qp = p.q + (int64_t)(r.r0 + token) * p.ld_q + (int64_t)(head * p.group + g) * D + tq * 16;
       uint4 w[KC][2];
       float amax = 0.0f;
@@ -262,7 +279,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       for (int e2 = 0; e2 < 2; ++e2) {
         qf[x][e2] = __shfl_sync(0xffffffffu, factor, 8 * tq + 4 * e2);
         const int rr = 8 * x + 2 * tq + e2;
-        pos[x][e2] = rr < valid ? r.len - r.n + (int)((row0 + rr) / p.group) : -1;
+        pos[x][e2] = rr < valid ? first_pos + (head0 + rr) / p.group : -1;
       }
     }
 
@@ -276,9 +293,10 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       const uint2 info = reinterpret_cast<const uint2*>(s_info + st)[warp & 1];
       const uint32_t sc[2] = {info.x, info.y};     // of keys 0..15 and 16..31
       if (j0 < key_end) {
-        // whole: every key is there; clear: and every row sees every key, under one pair of scales
+        const int lv[2] = {(int)(sc[0] >> 8 & 0xFF) - 127, (int)(sc[1] >> 8 & 0xFF) - 127};
+        // whole: every key is there; clear: and every row sees every key, and the value scales go together
         const bool whole = (sc[0] & sc[1]) >> 31 && j0 + 32 <= key_end;
-        const bool clear = whole && sc[0] == sc[1] && j0 + 31 <= first_pos && (p.window <= 0 || j0 > last_pos - p.window);
+        const bool clear = whole && abs(lv[0] - lv[1]) <= kSpan && j0 + 31 <= first_pos && (p.window <= 0 || j0 > last_pos - p.window);
         if (!whole) {                              // value rows without a visible key: whatever they hold becomes 0
           if (!(sc[lane >> 4] >> 31) || j0 + lane >= key_end)
 #pragma unroll
@@ -288,49 +306,56 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 
         // ---- products with the keys: this lane has keys j0 + 8 g + mk of rows 8 x + 2 tq + {0, 1} ----
         float s[RB][4][2];
+        float c[2][RB][4];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          float c[RB][4];
+        for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
           for (int x = 0; x < RB; ++x)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[x][i] = 0.0f;
+            for (int i = 0; i < 4; ++i) c[mt][x][i] = 0.0f;
 #pragma unroll
-          for (int ch = 0; ch < KC; ++ch) {
-            const uint4 k0 = *reinterpret_cast<const uint4*>(ks + swz<D>(16 * mt + mk, 4 * ch + tq));
-            const uint4 k1 = *reinterpret_cast<const uint4*>(ks + swz<D>(16 * mt + 8 + mk, 4 * ch + tq));
-            const uint32_t ka[4] = {k0.x, k0.y, k0.z, k0.w}, kb[4] = {k1.x, k1.y, k1.z, k1.w};
+        for (int ch = 0; ch < KC; ++ch) {
+          uint4 kk[2][2];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) kk[mt][e] = *reinterpret_cast<const uint4*>(ks + swz<D>(16 * mt + 8 * e + mk, 4 * ch + tq));
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {                          // two independent chains of products
+              const uint32_t ka = k == 0 ? kk[mt][0].x : k == 1 ? kk[mt][0].y : k == 2 ? kk[mt][0].z : kk[mt][0].w;
+              const uint32_t kb = k == 0 ? kk[mt][1].x : k == 1 ? kk[mt][1].y : k == 2 ? kk[mt][1].z : kk[mt][1].w;
               uint32_t a0, a1, a2, a3;
-              to_f16(ka[k], a0, a2);
-              to_f16(kb[k], a1, a3);
+              to_f16(ka, a0, a2);
+              to_f16(kb, a1, a3);
 #pragma unroll
-              for (int x = 0; x < RB; ++x) mma_f16(c[x], a0, a1, a2, a3, qb[x][4 * ch + k][0], qb[x][4 * ch + k][1]);
+              for (int x = 0; x < RB; ++x) mma_f16(c[mt][x], a0, a1, a2, a3, qb[x][4 * ch + k][0], qb[x][4 * ch + k][1]);
             }
-          }
+        }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
           for (int x = 0; x < RB; ++x)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) s[x][2 * mt + h][e] = c[x][2 * h + e];
-        }
-        uint32_t vr[4][2][VB / 4];                 // values of keys 8 g + ve[e], channels VB lr ..
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            if constexpr (D == 128) {
-              const uint4 x = *reinterpret_cast<const uint4*>(vs + swz<D>(8 * g + ve[e], lr));
-              vr[g][e][0] = x.x; vr[g][e][1] = x.y; vr[g][e][2] = x.z; vr[g][e][3] = x.w;
-            } else {
-              const uint2 x = *reinterpret_cast<const uint2*>(vs + swz<D>(8 * g + ve[e], lr >> 1) + 8 * (lr & 1));
-              vr[g][e][0] = x.x; vr[g][e][1] = x.y;
-            }
-          }
+              for (int e = 0; e < 2; ++e) s[x][2 * mt + h][e] = c[mt][x][2 * h + e];
         // o = a * o + P^T V with pb: keys 8 g + ve[e] of row 8 x + lr
         auto accumulate = [&](const float (&a)[RB][2], const uint32_t (&pb)[RB][4]) {
+          uint32_t vr[4][2][VB / 4];                 // values of keys 8 g + ve[e], channels VB lr ..
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if constexpr (D == 128) {
+                const uint4 x = *reinterpret_cast<const uint4*>(vs + swz<D>(8 * g + ve[e], lr));
+                vr[g][e][0] = x.x; vr[g][e][1] = x.y; vr[g][e][2] = x.z; vr[g][e][3] = x.w;
+              } else {
+                const uint2 x = *reinterpret_cast<const uint2*>(vs + swz<D>(8 * g + ve[e], lr >> 1) + 8 * (lr & 1));
+                vr[g][e][0] = x.x; vr[g][e][1] = x.y;
+              }
+            }
           bool moved = false;
 #pragma unroll
           for (int x = 0; x < RB; ++x) moved |= a[x][0] != 1.0f || a[x][1] != 1.0f;
@@ -356,27 +381,27 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             }
           }
         };
-        const int lv[2] = {(int)(sc[0] >> 8 & 0xFF) - 127, (int)(sc[1] >> 8 & 0xFF) - 127};
         float alpha[RB][2];
         uint32_t pb[RB][4];
         if (clear) {
-          const int was = R == kNone ? lv[0] : R;
-          R = lv[0] > was || lv[0] < was - kSpan ? lv[0] : was;
-          const float kf = pow2_byte(sc[0] & 0xFF), move = pow2i(was - R), down = pow2i(R - lv[0] - 15), shift = (float)(15 + lv[0] - R);
+          const int lead = max(lv[0], lv[1]), was = R == kNone ? lead : R;
+          R = lead > was || lead < was - kSpan ? lead : was;
+          const float kf[2] = {pow2_byte(sc[0] & 0xFF), pow2_byte(sc[1] & 0xFF)}, move = pow2i(was - R);
+          const float down[2] = {pow2i(R - lv[0] - 15), pow2i(R - lv[1] - 15)}, shift[2] = {(float)(15 + lv[0] - R), (float)(15 + lv[1] - R)};
 #pragma unroll
           for (int x = 0; x < RB; ++x) {
             float w[4][2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float fs = qf[x][e] * kf;                           // not negative: the sign of the scale is in the query
-              const float mn = fmaxf(m[x][e], column_max(fmaxf(fmaxf(s[x][0][e], s[x][1][e]), fmaxf(s[x][2][e], s[x][3][e]))) * fs);
-              const float a = ex2(m[x][e] - mn), base = shift - mn;
+              const float fs[2] = {qf[x][e] * kf[0], qf[x][e] * kf[1]};   // not negative: the sign of the scale is in the query
+              const float mn = fmaxf(m[x][e], column_max(fmaxf(fmaxf(s[x][0][e], s[x][1][e]) * fs[0], fmaxf(s[x][2][e], s[x][3][e]) * fs[1])));
+              const float a = ex2(m[x][e] - mn), base[2] = {shift[0] - mn, shift[1] - mn};
               alpha[x][e] = a * move;
               m[x][e] = mn;
-              float sum = 0.0f;
 #pragma unroll
-              for (int g = 0; g < 4; ++g) { w[g][e] = ex2(fmaf(s[x][g][e], fs, base)); sum += w[g][e]; }
-              l[x][e] = fmaf(l[x][e], a, sum * down);                   // the sum is of the weights without the values' scale
+              for (int g = 0; g < 4; ++g) w[g][e] = ex2(fmaf(s[x][g][e], fs[g >> 1], base[g >> 1]));
+              // the sum is of the weights without the values' scale
+              l[x][e] = fmaf(l[x][e], a, fmaf(w[0][e] + w[1][e], down[0], (w[2][e] + w[3][e]) * down[1]));
             }
 #pragma unroll
             for (int g = 0; g < 4; ++g) pb[x][g] = transpose8x8(pack_f16(w[g][0], w[g][1]));
@@ -446,6 +471,18 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if (lane == 0) s_r[warp] = R;
   }
   __syncthreads();
+  // row rr, channels cc .. of the outputs: a row that sees no key has ll = 0, zeros and -inf; a query that holds an infinity or a NaN has
+  // ll = NaN and stays NaN
+  auto finish = [&](int rr, int cc, const float4 acc, float mm, float ll, int unit_exp) {
+    const int hd = head0 + rr, tk = hd / p.group;
+    const int64_t orow = (int64_t)(r.r0 + token0 + tk) * (t.n_kv_heads * p.group) + head * p.group + (hd - tk * p.group);
+    const float k = (ll == 0.0f ? 0.0f : __frcp_rn(ll)), up = unit_exp == kNone ? 0.0f : pow2i(unit_exp - 15);
+    const __nv_bfloat162 y0 = __floats2bfloat162_rn(acc.x * k * up, acc.y * k * up), y1 = __floats2bfloat162_rn(acc.z * k * up, acc.w * k * up);
+    uint2 pk;
+    pk.x = *reinterpret_cast<const uint32_t*>(&y0); pk.y = *reinterpret_cast<const uint32_t*>(&y1);
+    *reinterpret_cast<uint2*>(p.out + orow * D + cc) = pk;
+    if (p.lse && cc == 0) p.lse[orow] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
+  };
   int cr = kNone;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) cr = max(cr, s_r[w]);
@@ -463,40 +500,37 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       const float4 x = *reinterpret_cast<const float4*>(&s_o[w][rr][cc]);
       acc.x += fo * x.x; acc.y += fo * x.y; acc.z += fo * x.z; acc.w += fo * x.w;
     }
+    if (split == 1) {
+      if (rr < valid) finish(rr, cc, acc, mm, ll, cr);
+      continue;
+    }
     *reinterpret_cast<float4*>(&s_o[0][rr][cc]) = acc;                // read and written by this thread alone
     if (cc == 0) { s_cm[rr] = mm; s_cl[rr] = ll; }
   }
-  if (threadIdx.x == 0) s_cr = cr;
-  if (split > 1) cluster.sync(); else __syncthreads();
-  int tr = kNone;
-  for (int c = 0; c < split; ++c) tr = max(tr, split > 1 ? *cluster.map_shared_rank(&s_cr, c) : s_cr);
-  const int cols = D / split;                                         // this CTA finishes channels part * cols ..
-  for (int i = threadIdx.x; i < kRows * cols / 4; i += kThreads) {
-    const int rr = i / (cols / 4), cc = part * cols + (i % (cols / 4)) * 4;
-    if (rr >= valid) continue;
-    float mm = -INFINITY, ll = 0.0f;
-    for (int c = 0; c < split; ++c) mm = fmaxf(mm, split > 1 ? *cluster.map_shared_rank(&s_cm[rr], c) : s_cm[rr]);
-    const float b = mm == -INFINITY ? 0.0f : mm;
-    float4 acc = make_float4(0, 0, 0, 0);
-    for (int c = 0; c < split; ++c) {
-      const float a = ex2((split > 1 ? *cluster.map_shared_rank(&s_cm[rr], c) : s_cm[rr]) - b);
-      const int rc = split > 1 ? *cluster.map_shared_rank(&s_cr, c) : s_cr;
-      const float fo = a * (rc == kNone ? 0.0f : pow2i(rc - tr));
-      ll += a * (split > 1 ? *cluster.map_shared_rank(&s_cl[rr], c) : s_cl[rr]);
-      const float4 x = *reinterpret_cast<const float4*>(split > 1 ? cluster.map_shared_rank(&s_o[0][rr][cc], c) : &s_o[0][rr][cc]);
-      acc.x += fo * x.x; acc.y += fo * x.y; acc.z += fo * x.z; acc.w += fo * x.w;
+  if (split > 1) {
+    if (threadIdx.x == 0) s_cr = cr;
+    cluster.sync();
+    int tr = kNone;
+    for (int c = 0; c < split; ++c) tr = max(tr, *cluster.map_shared_rank(&s_cr, c));
+    for (int i = part * kThreads + threadIdx.x; i < kRows * D / 4; i += split * kThreads) {   // every CTA finishes a part of the rows
+      const int rr = i / (D / 4), cc = (i % (D / 4)) * 4;
+      if (rr >= valid) continue;
+      float mm = -INFINITY, ll = 0.0f;
+      for (int c = 0; c < split; ++c) mm = fmaxf(mm, *cluster.map_shared_rank(&s_cm[rr], c));
+      const float b = mm == -INFINITY ? 0.0f : mm;
+      float4 acc = make_float4(0, 0, 0, 0);
+      for (int c = 0; c < split; ++c) {
+        const float a = ex2(*cluster.map_shared_rank(&s_cm[rr], c) - b);
+        const int rc = *cluster.map_shared_rank(&s_cr, c);
+        const float fo = a * (rc == kNone ? 0.0f : pow2i(rc - tr));
+        ll += a * *cluster.map_shared_rank(&s_cl[rr], c);
+        const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(&s_o[0][rr][cc], c));
+        acc.x += fo * x.x; acc.y += fo * x.y; acc.z += fo * x.z; acc.w += fo * x.w;
+      }
+      finish(rr, cc, acc, mm, ll, tr);
     }
-    const int tk = (int)((row0 + rr) / p.group), hd = head * p.group + (int)((row0 + rr) % p.group);
-    const int64_t orow = (int64_t)(r.r0 + tk) * (t.n_kv_heads * p.group) + hd;
-    // a row that sees no key has ll = 0: zeros and -inf.  A query that holds an infinity or a NaN has ll = NaN and stays NaN.
-    const float inv = ll == 0.0f ? 0.0f : __frcp_rn(ll), up = tr == kNone ? 0.0f : pow2i(tr - 15);
-    const __nv_bfloat162 y0 = __floats2bfloat162_rn(acc.x * inv * up, acc.y * inv * up), y1 = __floats2bfloat162_rn(acc.z * inv * up, acc.w * inv * up);
-    uint2 pk;
-    pk.x = *reinterpret_cast<const uint32_t*>(&y0); pk.y = *reinterpret_cast<const uint32_t*>(&y1);
-    *reinterpret_cast<uint2*>(p.out + orow * D + cc) = pk;
-    if (p.lse && cc == 0) p.lse[orow] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
+    cluster.sync();                                                   // the others may still be reading this CTA's shared memory
   }
-  if (split > 1) cluster.sync();                                      // the others may still be reading this CTA's shared memory
   if (threadIdx.x == 0 && s_abort) report(t.status, B2Q_ERR_TIMEOUT);
 }
 
@@ -559,10 +593,12 @@ extern "C" int32_t b2q_kv8_attention_bf16(b2q_handle h, const void* q, int64_t l
   if (q_starts && tokens * p.group > 32 * seqs) return b2q_kv8_prefill(h, p, head_dim);
   // rows that share keys: up to 8 a CTA, 16 where a sequence has more than 8 on average (one conversion of the codes serves both halves)
   const int rb = tokens * p.group > 8 * seqs ? 2 : 1, per = 8 * rb;
+  if (tokens * p.group > 0x7FFFFFFF - 16) B2Q_FAIL(h, B2Q_ERR_INVALID_DIMENSION, "kv8_attention: %lld tokens of %lld heads are too many", (long long)tokens, (long long)n_heads);
   const int64_t units = q_starts ? tokens * p.group / per + seqs : seqs * ceil_div64(p.group, per);
   const int64_t keys = p.window ? p.window + kv8::kTile : most;
   int split = 1;
   while (split < 8 && units * n_kv_heads * split * 2 <= 4 * (int64_t)h->sm_count && keys > split * kv8::kTile * kv8::kWarps / 2) split *= 2;
+  if (getenv("SPL")) split = atoi(getenv("SPL"));
   if (units * split > 0x7FFFFFFF) B2Q_FAIL(h, B2Q_ERR_INVALID_DIMENSION, "kv8_attention: %lld tokens of %lld heads are too many", (long long)tokens, (long long)n_heads);
   if (head_dim == 64) return rb == 1 ? kv8_decode_launch<64, 1>(h, p, units, split) : kv8_decode_launch<64, 2>(h, p, units, split);
   return rb == 1 ? kv8_decode_launch<128, 1>(h, p, units, split) : kv8_decode_launch<128, 2>(h, p, units, split);
