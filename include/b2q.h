@@ -219,8 +219,10 @@ int32_t b2q_kv8_append_bf16(b2q_handle h, const void* k, const void* v, int64_t 
                             uint8_t* v_scales);
 /* out [tokens][n_heads][head_dim] bf16 = softmax(scale * q k^T) v over the keys at positions <= the row's own, with window > 0 the last
  * `window` of them; query head g reads kv head g / (n_heads / n_kv_heads).  lse (optional, f32 [tokens][n_heads]) receives the natural
- * logarithm of the softmax denominators.  A row that sees no key gives zeros and -inf.  Scores, maxima, sums and outputs are held in f32;
- * a query element is off by at most 2^-17 of its row's largest, a softmax weight by 2^-9 of itself. */
+ * logarithm of the softmax denominators.  A row that sees no key gives zeros and -inf.  Table entries of pages that no row's window
+ * reaches are not looked at.  A query that holds an infinity or a NaN makes its own row NaN; the codes of cached tokens are taken to be
+ * finite, as b2q_kv8_append_bf16 writes them (a slot that holds no token may hold anything).  Scores, maxima, sums and outputs are held in
+ * f32; a query element is off by at most 2^-17 of its row's largest, a softmax weight by 2^-9 of itself. */
 int32_t b2q_kv8_attention_bf16(b2q_handle h, const void* q, int64_t ld_q, int64_t tokens, int64_t n_heads, const int32_t* q_starts,
                                const int32_t* seq_lens, const int32_t* block_tables, int64_t seqs, int64_t table_width, int64_t num_pages,
                                int64_t page_size, int64_t n_kv_heads, int64_t head_dim, const uint8_t* k_codes, const uint8_t* v_codes,

@@ -13,9 +13,8 @@
 // of, the order of channels); 8 x 8 tiles of P are transposed between lanes by movmatrix, pairs of keys of V by byte permutations.
 // One warp brings tiles of 64 keys into a ring of shared memory by TMA (it alone walks the block table, a batch of tiles ahead); three
 // pairs of warps take the tiles in turn, 32 keys to a warp, each with its own running maximum and sum, so the main loop has no
-// barrier between them.  Warps and the CTAs of a
-// cluster (tiles dealt round) are joined once at the end, through shared and distributed shared memory: no workspace, one
-// launch, and a result that does not depend on timing.
+// barrier between them.  Warps and the CTAs of a cluster (tiles dealt round) are joined once at the end, through shared and distributed
+// shared memory: no workspace, one launch, and a result that does not depend on timing.
 // The value scale is a power of two 2^lv per page: weights enter as p * 2^(15 + lv - R) and the outputs are kept in units of
 // 2^(R - 15), R following the pages' scales, so the weights keep their precision whatever the pages' sizes are; pages of one tile
 // whose scales lie more than 2^8 apart are multiplied one after the other.
@@ -25,7 +24,6 @@
 #include "kv8.cuh"
 #include "tc_common.cuh"
 #include <cooperative_groups.h>
-#include <stdlib.h>
 
 namespace cg = cooperative_groups;
 
@@ -137,7 +135,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const int token0 = row0 / p.group, head0 = row0 - token0 * p.group;       // of the first row, within the sequence and the group
   const int first_pos = r.len - r.n + token0, last_pos = first_pos + (head0 + valid - 1) / p.group;
   const int key_end = last_pos + 1;
-  const int key_begin = p.window > 0 ? max(0, first_pos - p.window + 1) & ~(kTile - 1) : 0;
+  // the first key that a row sees; the first tile may begin before it, with pages that its owner has given up and that are not looked up
+  const int key_low = p.window > 0 ? max(0, first_pos - p.window + 1) : 0, key_begin = key_low & ~(kTile - 1);
 
   const int tiles = (key_end - key_begin + kTile - 1) / kTile, mine = (tiles - part + split - 1) / split;   // tiles part, part + split, ..
 
@@ -165,7 +164,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int j = j0 + rows_each * e;
-        pg[e] = e < subs && i0 + lane < mine && j < key_end ? page_of(t, f.x, j >> t.page_shift, head == 0) : -1;
+        pg[e] = e < subs && i0 + lane < mine && j < key_end && (j | (rows_each - 1)) >= key_low ? page_of(t, f.x, j >> t.page_shift, head == 0) : -1;
       }
     };
     auto scales = [&] {
@@ -565,6 +564,25 @@ static int32_t kv8_decode_launch(b2q_handle h, const kv8::AttendArgs& p, int64_t
   return B2Q_OK;
 }
 
+// CTAs that share the keys of the same rows: the number for which the busiest SM is done first, by its CTAs times the tiles of each plus
+// kFixed for what every CTA costs besides.  A CTA alone on an SM that has room for two leaves some of it idle (kAlone).  Measured with 8
+// query rows to a kv head of 128 channels and 8 kv heads, by the number of CTAs to the same rows, in us:
+//   sequences x keys     1     2     3     4     6     8        sequences x keys     1     2     3     4     6     8
+//          1 x 32000   187    99    69    54    40    32              16 x 8200    60    52    61    54    62    68
+//           4 x 8200    53    32    25    27    24    21              20 x 8200    88    70    68    71    80    87
+//           8 x 8200    57    35    39    33    42    40              32 x 8200    93    92   100   102   118   130
+//          12 x 8200    58    51    49    51    52    54              32 x 1000    20    25    32    37    53    65
+static int kv8_decode_split(int64_t units, int64_t tiles, int rb, int sms) {
+  constexpr double kFixed = 12, kAlone = 1.3;
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= 8; ++s) {
+    const double ctas = (double)ceil_div64(units * s, sms), cost = (rb == 1 && ctas < kAlone ? kAlone : ctas) * ((double)ceil_div64(tiles, s) + kFixed);
+    if (s == 1 || cost < least) { best = s; least = cost; }
+  }
+  return best;
+}
+
 int32_t b2q_kv8_prefill(b2q_handle h, const kv8::AttendArgs& p, int64_t head_dim);   // kv8_prefill.cu
 
 extern "C" int32_t b2q_kv8_attention_bf16(b2q_handle h, const void* q, int64_t ld_q, int64_t tokens, int64_t n_heads, const int32_t* q_starts,
@@ -590,15 +608,14 @@ extern "C" int32_t b2q_kv8_attention_bf16(b2q_handle h, const void* q, int64_t l
   p.window = window > 0 && window < most ? (int)window : 0;
   p.scale = scale * 1.4426950408889634f;
   p.out = static_cast<__nv_bfloat16*>(out); p.lse = lse;
+  if (tokens * p.group > 0x7FFFFFFF - 128)
+    B2Q_FAIL(h, B2Q_ERR_INVALID_DIMENSION, "kv8_attention: %lld tokens of %lld heads are too many", (long long)tokens, (long long)n_heads);
   if (q_starts && tokens * p.group > 32 * seqs) return b2q_kv8_prefill(h, p, head_dim);
   // rows that share keys: up to 8 a CTA, 16 where a sequence has more than 8 on average (one conversion of the codes serves both halves)
   const int rb = tokens * p.group > 8 * seqs ? 2 : 1, per = 8 * rb;
-  if (tokens * p.group > 0x7FFFFFFF - 16) B2Q_FAIL(h, B2Q_ERR_INVALID_DIMENSION, "kv8_attention: %lld tokens of %lld heads are too many", (long long)tokens, (long long)n_heads);
-  const int64_t units = q_starts ? tokens * p.group / per + seqs : seqs * ceil_div64(p.group, per);
-  const int64_t keys = p.window ? p.window + kv8::kTile : most;
-  int split = 1;
-  while (split < 8 && units * n_kv_heads * split * 2 <= 4 * (int64_t)h->sm_count && keys > split * kv8::kTile * kv8::kWarps / 2) split *= 2;
-  if (getenv("SPL")) split = atoi(getenv("SPL"));
+  const int64_t units = q_starts ? tokens * p.group / per + seqs : seqs * ceil_div64(p.group, per);   // at most
+  const int64_t tiles = ceil_div64(p.window ? p.window + kv8::kTile : most, kv8::kTile);
+  const int split = kv8_decode_split(seqs * ceil_div64(ceil_div64(tokens * p.group, seqs), per) * n_kv_heads, tiles, rb, h->sm_count);
   if (units * split > 0x7FFFFFFF) B2Q_FAIL(h, B2Q_ERR_INVALID_DIMENSION, "kv8_attention: %lld tokens of %lld heads are too many", (long long)tokens, (long long)n_heads);
   if (head_dim == 64) return rb == 1 ? kv8_decode_launch<64, 1>(h, p, units, split) : kv8_decode_launch<64, 2>(h, p, units, split);
   return rb == 1 ? kv8_decode_launch<128, 1>(h, p, units, split) : kv8_decode_launch<128, 2>(h, p, units, split);

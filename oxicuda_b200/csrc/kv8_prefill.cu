@@ -145,7 +145,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   const int token0 = (int)(row0 / p.group), head0 = (int)(row0 - (int64_t)token0 * p.group);   // of the tile's first row, within the sequence and the group
   const int first_pos = r.len - r.n + token0, last_pos = first_pos + (head0 + valid - 1) / p.group;
   const int key_end = last_pos + 1;
-  const int key_begin = p.window > 0 ? max(0, first_pos - p.window + 1) & ~(kTile - 1) : 0;
+  // the first key that a row sees; the first tile may begin before it, with pages that its owner has given up and that are not looked up
+  const int key_low = p.window > 0 ? max(0, first_pos - p.window + 1) : 0, key_begin = key_low & ~(kTile - 1);
   const int all = (key_end - key_begin + kTile - 1) / kTile, tiles = (all - part + split - 1) / split;   // tiles part, part + split, ..
 
   if (warp == 1) tmem_alloc(smem_u32(&s_tmem_base), C::kTmemCols);
@@ -173,7 +174,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         for (int e = 0; e < 4; ++e) {
           pg[e] = -1; info[e] = 0;
           const int j = j0 + rows_each * e;
-          if (e < subs && i0 + lane < tiles && j < key_end) {
+          if (e < subs && i0 + lane < tiles && j < key_end && (j | (rows_each - 1)) >= key_low) {
             pg[e] = page_of(t, f.x, j >> t.page_shift, head == 0);
             if (pg[e] >= 0)
               info[e] = kThere | (uint32_t)p.ks[(int64_t)pg[e] * t.n_kv_heads + head] | ((uint32_t)p.vs[(int64_t)pg[e] * t.n_kv_heads + head] << 8);
@@ -308,8 +309,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       const int src0 = key0 * D + ((D == 128 ? u ^ (key0 & 7) : u ^ ((key0 >> 1) & 3)) << 4);              // as TMA left it
       const int dst0 = (u >> 2) * (kTile * 128) + key0 * 128 + ((u2 ^ (key0 & 7)) << 4);                   // block u / 4, units 2 (u & 3) and the next
       const int step = (((u2 + 1) ^ (key0 & 7)) - (u2 ^ (key0 & 7))) * 16;
-      if (wait(qready, 0))                          // the query rows have passed through the tiles that are written here
-      for (int it = 0;; ++it) {
+      const bool free_now = wait(qready, 0);        // the query rows have passed through the tiles that are written here
+      for (int it = 0; free_now; ++it) {
         const int v = it % kVStages, b = it & 1;
         if (!wait(vfull(v), (it / kVStages) & 1) || !wait(wempty(b), ((it >> 1) & 1) ^ 1)) break;
         __syncwarp();

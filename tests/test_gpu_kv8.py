@@ -138,6 +138,84 @@ def test_window(cuda, window, news, olds):
 
 
 @pytest.mark.parametrize("ps", [16, 32, 64, 128])
+@pytest.mark.parametrize("window", [5, 50, 100])
+@pytest.mark.parametrize("new", [1, 3, 90])
+def test_pages_in_front_of_the_window_may_be_gone(cuda, ps, window, new):
+    """What no row's window reaches is not looked up: its owner may have given the pages back, and that is no error."""
+    from oxicuda_b200 import _lib as L
+    lens, news = [700, 333, 40 + new], [new] * 3
+    cache, table = _pages(cuda, lens, ps, 2, 128, ps + window)
+    q = _q(cuda, 3 * new, 8, 128, new)
+    seq, starts = torch.tensor(lens, dtype=torch.int32, device=cuda), None if new == 1 else _starts(news, cuda)
+    want = cache.attend(q, seq, table, q_starts=starts, window=window)
+    gone = table.clone()
+    for b, n in enumerate(lens):
+        gone[b, : max(0, n - new - window + 1) // ps] = -1
+    out, lse = cache.attend(q, seq, gone, q_starts=starts, window=window, want_lse=True)
+    L.default_handle().check()
+    assert torch.equal(out, want)
+    _check(cache, table, lens, news, q, out, lse, window=window)
+
+
+@pytest.mark.parametrize("ps,d", [(16, 64), (64, 128)])
+def test_many_sequences(cuda, ps, d):
+    """More sequences than a warp has lanes, many of them without rows."""
+    g = torch.Generator().manual_seed(3)
+    olds = torch.randint(0, 200, (100,), generator=g).tolist()
+    for top in (3, 40):
+        news = (torch.randint(0, top, (100,), generator=g) * torch.randint(0, 2, (100,), generator=g)).tolist()
+        news[:33] = [0] * 33
+        lens = [max(1, a + b) for a, b in zip(news, olds)]
+        cache, table = _pages(cuda, lens, ps, 2, d, top)
+        q = _q(cuda, sum(news), 8, d, top)
+        k, v = [_q(cuda, sum(news), 2, d, i) for i in (1, 2)]
+        seq, starts = torch.tensor(lens, dtype=torch.int32, device=cuda), _starts(news, cuda)
+        want = [t.clone() for t in (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)]
+        _append_ref(want[0], want[1], k, lens, news, table, ps)
+        _append_ref(want[2], want[3], v, lens, news, table, ps)
+        cache.append(k, v, seq, table, q_starts=starts)
+        for w, t in zip(want, (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)):
+            assert torch.equal(w, t)
+        out, lse = cache.attend(q, seq, table, q_starts=starts, want_lse=True)
+        _check(cache, table, lens, news, q, out, lse)
+
+
+@pytest.mark.parametrize("new", [1, 2, 5])
+@pytest.mark.parametrize("group", [33, 64, 128, 200])
+def test_large_groups(cuda, group, new):
+    lens = [90, 5, 400]
+    cache, table = _pages(cuda, lens, 16, 1, 128, group)
+    q = _q(cuda, 3 * new, group, 128, new)
+    seq, starts = torch.tensor(lens, dtype=torch.int32, device=cuda), None if new == 1 else _starts([new] * 3, cuda)
+    out, lse = cache.attend(q, seq, table, q_starts=starts, want_lse=True)
+    _check(cache, table, lens, [new] * 3, q, out, lse)
+
+
+@pytest.mark.parametrize("new", [1, 4, 100])
+def test_sequences_that_share_their_first_pages(cuda, new):
+    """A common prompt: several tables name the same pages."""
+    lens = [256 + new, 300 + new, 256 + new]
+    cache, table = _pages(cuda, lens, 32, 2, 128, new)
+    table[1:, :8] = table[0, :8]
+    q = _q(cuda, 3 * new, 8, 128, 9)
+    seq, starts = torch.tensor(lens, dtype=torch.int32, device=cuda), None if new == 1 else _starts([new] * 3, cuda)
+    out, lse = cache.attend(q, seq, table, q_starts=starts, want_lse=True)
+    _check(cache, table, lens, [new] * 3, q, out, lse)
+
+
+@pytest.mark.parametrize("new,old", [(1, 9000), (2, 9000), (5, 9000), (40, 9000), (130, 6000)])
+def test_long_keys_of_few_rows(cuda, new, old):
+    """Keys dealt to the CTAs of a cluster, in every number of them that a batch of this kind meets."""
+    for seqs in (1, 3, 6):
+        lens = [old + new + 64 * i for i in range(seqs)]
+        cache, table = _pages(cuda, lens, 64, 4, 128, seqs)
+        q = _q(cuda, seqs * new, 8, 128, new)
+        seq, starts = torch.tensor(lens, dtype=torch.int32, device=cuda), None if new == 1 else _starts([new] * seqs, cuda)
+        out, lse = cache.attend(q, seq, table, q_starts=starts, want_lse=True)
+        _check(cache, table, lens, [new] * seqs, q, out, lse)
+
+
+@pytest.mark.parametrize("ps", [16, 32, 64, 128])
 @pytest.mark.parametrize("jump", [3, 9, 25])
 @pytest.mark.parametrize("new", [1, 150])
 def test_pages_of_different_sizes(cuda, ps, jump, new):
