@@ -48,7 +48,7 @@ template <int D> struct Cfg {
   static constexpr int kTileBytes = kTile * D;
   static constexpr int kV16 = 2 * kTileBytes;    // a value tile in f16: D / 64 blocks of 64 keys x 128 bytes
   static constexpr int kData = kQ + (kKStages + kVStages) * kTileBytes + 2 * kV16;
-  static constexpr int kSmem = kData + 1024 + kInfo * 32 + 256;
+  static constexpr int kSmem = kData + 1024 + kInfo * 80 + 256;
   static constexpr int kTmemCols = 256;          // S: 2 x 64, O: D
   static_assert(kRows * D * 4 <= kData, "the join reuses the tiles");
 };
@@ -89,7 +89,27 @@ __device__ __forceinline__ uint32_t pack16(uint16_t lo, uint16_t hi) { return (u
 constexpr uint64_t kOne2 = 0x3F8000003F800000ull;   // 1.0f twice
 __device__ __forceinline__ uint64_t dup(float x) { return (uint64_t)__float_as_uint(x) << 32 | __float_as_uint(x); }
 
-struct Info { uint32_t w[4]; int j0, last; };    // per 16 keys: scales and flags; first key; 1 for the last tile
+// A tile, as the producer describes it to the others; per 16 keys and of the tile.  R follows the pages' value scales 2^lv: weights enter
+// as p * 2^up, a sum of them counts 2^down, O is in units of 2^(R - 8) and moves by the factor `move` to this tile's.
+struct __align__(16) Info {
+  uint32_t flags[4];
+  float kf[4], up[4], down[4];                   // the keys' scale, 8 + lv - R, 2^(R - lv - 8)
+  int j0, last, R;                               // first key; 1 for the last tile
+  float move;
+};
+// three at a time
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// what the last tmem_ld32 into r waits for, and no use of r before it
+__device__ __forceinline__ void landed(uint32_t (&r)[64]) {
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 64; i += 8)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -107,8 +127,9 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   auto wfull = [&](int b) { return more + 8u * b; };          // f16 value tiles
   auto wempty = [&](int b) { return more + 8u * (2 + b); };
   auto sfull = [&](int b) { return more + 8u * (4 + b); };
-  const uint32_t qready = more + 48, pfull = more + 56, pvdone = more + 64, drain = more + 72;
-  Info* const s_info = reinterpret_cast<Info*>(smem + (bar_at - base) + 8 * (2 * kKStages + 2 * kVStages + 10));
+  auto pfull = [&](int b) { return more + 8u * (6 + b); };    // the softmax may be a tile ahead of the products: a barrier for each S
+  const uint32_t qready = more + 64, pvdone = more + 72, drain = more + 80, odone = more + 88;
+  Info* const s_info = reinterpret_cast<Info*>(smem + (bar_at - base) + 8 * (2 * kKStages + 2 * kVStages + 12));   // 22 barriers in front
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
   __shared__ float s_m[kRows], s_l[kRows];        // score factors of the rows; for the join this CTA's maxima, sums and units
@@ -122,7 +143,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     for (int s = 0; s < kKStages; ++s) { mbar_init(kfull(s), 1); mbar_init(kempty(s), 1); }
     for (int s = 0; s < kVStages; ++s) { mbar_init(vfull(s), 1); mbar_init(vempty(s), 2); }
     for (int b = 0; b < 2; ++b) { mbar_init(wfull(b), 2); mbar_init(wempty(b), 1); mbar_init(sfull(b), 1); }
-    mbar_init(qready, 4); mbar_init(pfull, 4); mbar_init(pvdone, 1); mbar_init(drain, 1);
+    mbar_init(qready, 7); mbar_init(pfull(0), 4); mbar_init(pfull(1), 4); mbar_init(pvdone, 1); mbar_init(drain, 1); mbar_init(odone, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_k)) : "memory");
@@ -147,7 +168,28 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   const int key_end = last_pos + 1;
   // the first key that a row sees; the first tile may begin before it, with pages that its owner has given up and that are not looked up
   const int key_low = p.window > 0 ? max(0, first_pos - p.window + 1) : 0, key_begin = key_low & ~(kTile - 1);
-  const int all = (key_end - key_begin + kTile - 1) / kTile, tiles = (all - part + split - 1) / split;   // tiles part, part + split, ..
+  const int all = (key_end - key_begin + kTile - 1) / kTile;
+  int tiles = (all - part + split - 1) / split;   // tiles part, part + split, ..
+
+  // ---------------- the query rows, by warps 1 .. 7: D / 8 lanes to a row, 8 channels each, so that a warp reads whole rows ----------------
+  // They come in through the space of the f16 value tiles (free until the first of those is made), and a short loop turns them: unrolled
+  // over registers the same work was 13 KB of code that every CTA fetched once, 7 us.
+  constexpr int LPR = D / 8, RPW = 32 / LPR, QI = (kRows / RPW + 6) / 7;      // lanes to a row, rows at once, turns of a warp
+  static_assert(QI * RPW <= 32, "a lane holds the address of each row");
+  const int qc = lane % LPR;                                                  // 16 bytes of bf16 = half a 16-byte unit of codes
+  uint8_t* const raw = smem + (w_at - base);
+  auto qrow_of = [&](int i, int j) { return RPW * (warp - 1 + 7 * i) + j; };  // row j of turn i
+  if (warp > 0) {
+    const int mine = qrow_of(lane / RPW, lane % RPW);
+    const int hr = head0 + (mine < valid ? mine : 0);                         // rows behind the last one: the first row's
+    const __nv_bfloat16* const at = p.q + (int64_t)(r.r0 + token0 + hr / p.group) * p.ld_q + (int64_t)(head * p.group + hr % p.group) * D;
+#pragma unroll 1
+    for (int i = 0; i < QI; ++i) {
+      const int rr = qrow_of(i, lane / LPR);
+      const unsigned long long from = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), i * RPW + lane / LPR) + 16 * qc;
+      if (rr < kRows) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(raw + rr * (2 * D) + 16 * qc)), "l"(from) : "memory");
+    }
+  }
 
   if (warp == 1) tmem_alloc(smem_u32(&s_tmem_base), C::kTmemCols);
   tc_fence_before();
@@ -158,6 +200,45 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   const uint32_t tmem = s_tmem_base, tmem_o = tmem + 2 * kTile;
   volatile int* abort_flag = &s_abort;
   auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, abort_flag, kWaitLimitNs, 1); };
+
+  if (warp > 0) {
+    const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < QI; ++i) {
+      const int rr = qrow_of(i, lane / LPR), from = min(rr, kRows - 1);
+      const uint4 w = *reinterpret_cast<const uint4*>(raw + from * (2 * D) + 16 * qc);
+      const __nv_bfloat162* const q2 = reinterpret_cast<const __nv_bfloat162*>(&w);
+      // the largest of the row, a NaN if it holds one
+      __nv_bfloat162 top = __hmax2_nan(__hmax2_nan(__habs2(q2[0]), __habs2(q2[1])), __hmax2_nan(__habs2(q2[2]), __habs2(q2[3])));
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) top = __hmax2_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float amax = __bfloat162float(__hmax_nan(top.x, top.y));
+      const uint32_t u = __float_as_uint(amax);
+      const int e = max(-119, (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0));
+      const float inv = sign * pow2i(-e);
+      uint16_t h[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {                                            // exact in f16 down to 2^-24
+        const float2 x = __bfloat1622float2(q2[j]);
+        split_f16(pack_f16(x.x * inv, x.y * inv), h[j], l[j]);
+      }
+      if (rr < kRows) {
+        // rows of 128 bytes, 128-byte swizzle; 64 channels: both terms share a row
+        uint8_t* const qrow = smem + rr * 128;
+        const int unit16 = qc >> 1, in16 = (qc & 1) * 8;
+        *reinterpret_cast<uint2*>(qrow + ((unit16 ^ (rr & 7)) << 4) + in16) = make_uint2(pack16(h[0], h[1]), pack16(h[2], h[3]));
+        *reinterpret_cast<uint2*>(qrow + (D == 128 ? kRows * 128 + ((unit16 ^ (rr & 7)) << 4) : ((unit16 + 4) ^ (rr & 7)) << 4) + in16) =
+            make_uint2(pack16(l[0], l[1]), pack16(l[2], l[3]));
+        // a query with an infinity or a NaN: NaN throughout
+        if (qc == 0) s_m[rr] = amax < INFINITY ? fabsf(p.scale) * pow2i(e) : __uint_as_float(0x7FC00000u);
+      }
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(qready);
+  }
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFirst));
@@ -182,7 +263,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
       };
       bool ok = true;
-      int it = 0;                                   // tiles issued: a tile is walked once per group of pages whose value scales are alike
+      int R = kNone, it = 0;                        // tiles issued: a tile is walked once per group of pages whose value scales are alike
       fetch(0);
       for (int i0 = 0; i0 < tiles && ok; i0 += 32) {
         int cp[4];
@@ -217,14 +298,24 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             if (lane == 0) {
               ok = wait(kempty(s), ((it / kKStages) & 1) ^ 1);
               if (ok) {
-                Info d;
+                const int was = R == kNone ? lead + kRoom : R;
+                R = lead == kNone ? R : lead > was || lead < was - kSpan ? lead + kRoom : was;
+                Info* const d = &s_info[it % kInfo];
+                uint32_t fl[4];
+                float kf[4], up[4], down[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                  const int src = e / (4 / subs);
-                  d.w[e] = f4[src] | (take >> src & 1 ? kTaken : 0u);
+                  const int src = e / (4 / subs), lv = (int)(f4[src] >> 8 & 0xFF) - 127;
+                  fl[e] = (f4[src] & kThere) | (take >> src & 1 ? kTaken : 0u);
+                  kf[e] = pow2_byte(f4[src] & 0xFF);
+                  up[e] = (float)(8 + lv - R);
+                  down[e] = pow2i(R - lv - 8);
                 }
-                d.j0 = j; d.last = i0 + i == tiles - 1 && !rem;
-                s_info[it % kInfo] = d;
+                *reinterpret_cast<uint4*>(d->flags) = make_uint4(fl[0], fl[1], fl[2], fl[3]);
+                *reinterpret_cast<float4*>(d->kf) = make_float4(kf[0], kf[1], kf[2], kf[3]);
+                *reinterpret_cast<float4*>(d->up) = make_float4(up[0], up[1], up[2], up[3]);
+                *reinterpret_cast<float4*>(d->down) = make_float4(down[0], down[1], down[2], down[3]);
+                *reinterpret_cast<int4*>(&d->j0) = make_int4(j, i0 + i == tiles - 1 && !rem, R, __float_as_int(R == kNone ? 1.0f : pow2i(was - R)));
                 int there = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) there += p4[e] >= 0;
@@ -281,7 +372,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           // S of tile it + 1 overwrites S and P of tile it - 1: their product has to be done
           if (!last && !(ok = (it == 0 || wait(pvdone, (it - 1) & 1)) && scores(it + 1))) break;
           const int b = it & 1;
-          if (!wait(wfull(b), (it >> 1) & 1) || !wait(pfull, it & 1)) { ok = false; break; }
+          if (!wait(wfull(b), (it >> 1) & 1) || !wait(pfull(b), (it >> 1) & 1)) { ok = false; break; }
           tc_fence_after();
           const uint32_t vt = w_at + b * C::kV16;
           // 16 keys a step: two groups of 8 rows of 128 bytes; blocks of 64 channels lie 64 rows apart (leading byte offset)
@@ -292,7 +383,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           }
           tc_commit(wempty(b));
           tc_commit(pvdone);
-          if (last) break;
+          if (last) { tc_commit(odone); break; }
         }
         if (!ok) {
           tc_commit(drain);
@@ -314,16 +405,18 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const int v = it % kVStages, b = it & 1;
         if (!wait(vfull(v), (it / kVStages) & 1) || !wait(wempty(b), ((it >> 1) & 1) ^ 1)) break;
         __syncwarp();
-        const Info d = s_info[it % kInfo];
+        const Info& d = s_info[it % kInfo];
+        const uint32_t flags[4] = {d.flags[0], d.flags[1], d.flags[2], d.flags[3]};
+        const int j0 = d.j0, last = d.last;
         const uint8_t* const src = smem + (v_at - base) + v * C::kTileBytes + src0;
         uint8_t* const dst = smem + (w_at - base) + b * C::kV16 + dst0;
-        const bool whole = (d.w[0] & d.w[1] & d.w[2] & d.w[3]) >> 31 && d.j0 + kTile <= key_end;
+        const bool whole = (flags[0] & flags[1] & flags[2] & flags[3]) >> 31 && j0 + kTile <= key_end;
 #pragma unroll
         for (int k = 0; k < kTile; k += KEYS) {
           const uint4 x = *reinterpret_cast<const uint4*>(src + k * D);
           uint32_t o[8];
           to_f16(x.x, o[0], o[1]); to_f16(x.y, o[2], o[3]); to_f16(x.z, o[4], o[5]); to_f16(x.w, o[6], o[7]);
-          if (!whole && (!(d.w[(key0 + k) >> 4] & kThere) || d.j0 + key0 + k >= key_end))   // no visible key here: whatever the row holds becomes 0
+          if (!whole && (!(d.flags[(key0 + k) >> 4] & kThere) || j0 + key0 + k >= key_end))   // no visible key here: whatever the row holds becomes 0
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = 0;
           *reinterpret_cast<uint4*>(dst + k * 128) = make_uint4(o[0], o[1], o[2], o[3]);
@@ -332,7 +425,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         fence_async_smem();
         __syncwarp();
         if (lane == 0) { mbar_arrive(vempty(v)); mbar_arrive(wfull(b)); }
-        if (d.last) break;
+        if (last) break;
       }
     }
   } else {
@@ -343,114 +436,72 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     const bool live = row < valid;
     const int token = live ? token0 + (head0 + row) / p.group : 0, qhead = head * p.group + (live ? (head0 + row) % p.group : 0);
     const int pos = live ? r.len - r.n + token : -1;
-    {
-      // D / 8 lanes to a row, 8 channels each, so that a warp reads whole rows
-      constexpr int LPR = D / 8, RPW = 32 / LPR;
-      const int c = lane % LPR;                                              // 16 bytes of bf16 = half a 16-byte unit of codes
-      const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
-      const __nv_bfloat16* const mine = p.q + (int64_t)(r.r0 + token) * p.ld_q + (int64_t)qhead * D;   // rows behind the last one: the first row's
-      // The warp's rows come in through the space of its f16 value tiles (free until the first of them is made), and a short loop turns
-      // them: unrolled over registers the same work was 13 KB of code that every CTA fetched once, 7 us.
-      uint8_t* const raw = smem + (w_at - base) + quarter * 32 * (2 * D);
-#pragma unroll 1
-      for (int i = 0; i < 32; i += RPW) {
-        const int e = i + lane / LPR;
-        const unsigned long long from = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), e) + 16 * c;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(raw + e * (2 * D) + 16 * c)), "l"(from) : "memory");
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      __syncwarp();
-#pragma unroll 2
-      for (int i = 0; i < 32; i += RPW) {
-        const int e0 = i + lane / LPR, rr = quarter * 32 + e0;
-        const uint4 w = *reinterpret_cast<const uint4*>(raw + e0 * (2 * D) + 16 * c);
-        const __nv_bfloat162* const q2 = reinterpret_cast<const __nv_bfloat162*>(&w);
-        // the largest of the row, a NaN if it holds one
-        __nv_bfloat162 top = __hmax2_nan(__hmax2_nan(__habs2(q2[0]), __habs2(q2[1])), __hmax2_nan(__habs2(q2[2]), __habs2(q2[3])));
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) top = __hmax2_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float amax = __bfloat162float(__hmax_nan(top.x, top.y));
-        const uint32_t u = __float_as_uint(amax);
-        const int e = max(-119, (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0));
-        const float inv = sign * pow2i(-e);
-        uint16_t h[4], l[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {                                        // exact in f16 down to 2^-24
-          const float2 x = __bfloat1622float2(q2[j]);
-          split_f16(pack_f16(x.x * inv, x.y * inv), h[j], l[j]);
-        }
-        // rows of 128 bytes, 128-byte swizzle; 64 channels: both terms share a row
-        uint8_t* const qrow = smem + rr * 128;
-        const int unit16 = c >> 1, in16 = (c & 1) * 8;
-        *reinterpret_cast<uint2*>(qrow + ((unit16 ^ (rr & 7)) << 4) + in16) = make_uint2(pack16(h[0], h[1]), pack16(h[2], h[3]));
-        *reinterpret_cast<uint2*>(qrow + (D == 128 ? kRows * 128 + ((unit16 ^ (rr & 7)) << 4) : ((unit16 + 4) ^ (rr & 7)) << 4) + in16) =
-            make_uint2(pack16(l[0], l[1]), pack16(l[2], l[3]));
-        // a query with an infinity or a NaN: NaN throughout
-        if (c == 0) s_m[rr] = amax < INFINITY ? fabsf(p.scale) * pow2i(e) : __uint_as_float(0x7FC00000u);
-      }
-    }
-    fence_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(qready);
+    if (!wait(qready, 0)) tiles = -1;               // only if another warp has given up
     const float qf = s_m[row];
 
     float m = -INFINITY, l = 0.0f;
     int R = kNone;
-    bool ok = true;
-    int it = 0;
-    for (; tiles > 0; ++it) {
+    bool ok = tiles >= 0;
+    for (int it = 0; ok && tiles > 0; ++it) {
       const int b = it & 1;
+      const Info* const d = &s_info[it % kInfo];
       if (!wait(sfull(b), (it >> 1) & 1)) { ok = false; break; }
       __syncwarp();
       tc_fence_after();
-      const Info d = s_info[it % kInfo];
-      const bool whole = (d.w[0] & d.w[1] & d.w[2] & d.w[3]) >> 31 && d.j0 + kTile <= key_end;   // every key is there
-      // and every row sees every key (tile edges, windows and tiles walked in parts are masked)
-      const bool clear = whole && d.w[0] & d.w[1] & d.w[2] & d.w[3] & kTaken && d.j0 + kTile - 1 <= first_pos && (p.window <= 0 || d.j0 > last_pos - p.window);
-      // Masking rewrites S in TMEM, 16 columns at a time in a loop that stays rolled: as straight code between the load and its use it ran
-      // once or twice per CTA and cost it 8 us each time in instruction fetches.
+      uint32_t sr[64];
+      tmem_ld32(tmem + b * kTile + lanes, *reinterpret_cast<uint32_t(*)[32]>(&sr[0]));
+      tmem_ld32(tmem + b * kTile + 32 + lanes, *reinterpret_cast<uint32_t(*)[32]>(&sr[32]));
+      float fs[4], mt = -INFINITY;
+      const float4 kf = *reinterpret_cast<const float4*>(d->kf), up = *reinterpret_cast<const float4*>(d->up), down = *reinterpret_cast<const float4*>(d->down);
+      const int4 rest = *reinterpret_cast<const int4*>(&d->j0);
+      // not negative: the sign of the scale is in the query; not zero: -inf * 0 would be a NaN
+      fs[0] = qf * kf.x; fs[1] = qf * kf.y; fs[2] = qf * kf.z; fs[3] = qf * kf.w;
+      // clear: every row sees every key (tile edges, windows and tiles walked in parts are masked)
+      const uint32_t both = d->flags[0] & d->flags[1] & d->flags[2] & d->flags[3];
+      const bool clear = (both & (kThere | kTaken)) == (kThere | kTaken) && rest.x + kTile - 1 <= first_pos && (p.window <= 0 || rest.x > last_pos - p.window);
+      landed(sr);
+      // Masking rewrites S in TMEM, 16 columns at a time in a loop that stays rolled, and loads it again: as straight code between the load
+      // and its use it ran once or twice per CTA and cost it 8 us each time in instruction fetches.
       if (!clear) {
-        const int top = pos - d.j0, low = p.window > 0 ? top - p.window : -1;      // columns low < j <= top
+        const int top = pos - rest.x, low = p.window > 0 ? top - p.window : -1;      // columns low < j <= top
 #pragma unroll 1
         for (int c = 0; c < kTile; c += 16) {
           uint32_t x[16];
           tmem_ld16(tmem + b * kTile + c + lanes, x);
           tmem_ld_wait();
-          const int t2 = (s_info[it % kInfo].w[c >> 4] & kTaken ? top : -1) - c, l2 = low - c;
+          const int t2 = (d->flags[c >> 4] & kTaken ? top : -1) - c, l2 = low - c;
 #pragma unroll
           for (int j = 0; j < 16; ++j) if (j > t2 || j <= l2) x[j] = 0xFF800000u;
           tmem_st16(tmem + b * kTile + c + lanes, x);
         }
         tmem_st_wait();
+        tmem_ld32(tmem + b * kTile + lanes, *reinterpret_cast<uint32_t(*)[32]>(&sr[0]));
+        tmem_ld32(tmem + b * kTile + 32 + lanes, *reinterpret_cast<uint32_t(*)[32]>(&sr[32]));
+        landed(sr);
       }
-      uint32_t sr[64];
-      tmem_ld32(tmem + b * kTile + lanes, *reinterpret_cast<uint32_t(*)[32]>(&sr[0]));
-      tmem_ld32(tmem + b * kTile + 32 + lanes, *reinterpret_cast<uint32_t(*)[32]>(&sr[32]));
-      tmem_ld_wait();
-      int lead = kNone;
-      float fs[4], mt = -INFINITY;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        if (d.w[g] & kTaken) lead = max(lead, (int)(d.w[g] >> 8 & 0xFF) - 127);
-        // not negative: the sign of the scale is in the query; not zero: -inf * 0 would be a NaN
-        fs[g] = qf * pow2_byte(d.w[g] & 0xFF);
         fs[g] = fs[g] == 0.0f ? 1.17549435e-38f : fs[g];
-        float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float x[2];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j & 3] = fmaxf(x[j & 3], __uint_as_float(sr[16 * g + j]));
-        mt = fmaxf(mt, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * fs[g]);
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t* const y = sr + 16 * g + 8 * k;
+          x[k] = max3(__uint_as_float(y[0]), __uint_as_float(y[1]), __uint_as_float(y[2]));
+          x[k] = max3(x[k], __uint_as_float(y[3]), __uint_as_float(y[4]));
+          x[k] = max3(x[k], __uint_as_float(y[5]), __uint_as_float(y[6]));
+          x[k] = fmaxf(x[k], __uint_as_float(y[7]));
+        }
+        mt = fmaxf(mt, fmaxf(x[0], x[1]) * fs[g]);
       }
-      const int was = R == kNone ? lead + kRoom : R;
-      R = lead == kNone ? R : lead > was || lead < was - kSpan ? lead + kRoom : was;
       float alpha = 1.0f;
       if (mt > m + kSlack || (m == -INFINITY && mt > -INFINITY)) { alpha = ex2(m - mt); m = mt; }
       l *= alpha;
       const float back = m == -INFINITY ? 0.0f : m;   // a row that has seen nothing yet: exp2(-inf - 0) = 0
       uint32_t pw[32];
+      const float ups[4] = {up.x, up.y, up.z, up.w}, downs[4] = {down.x, down.y, down.z, down.w};
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int lv = (int)(d.w[g] >> 8 & 0xFF) - 127;
-        const uint64_t f2 = dup(fs[g]), add2 = dup((float)(8 + lv - R) - back);
+        const uint64_t f2 = dup(fs[g]), add2 = dup(ups[g] - back);
         uint64_t sum = 0;
 #pragma unroll
         for (int j = 16 * g; j < 16 * g + 16; j += 2) {
@@ -460,14 +511,17 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           fma2(sum, (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x), kOne2);
           pw[j >> 1] = pack_f16(x, y);
         }
-        l = fmaf(__uint_as_float((uint32_t)sum) + __uint_as_float((uint32_t)(sum >> 32)), pow2i(R - lv - 8), l);   // the weights without the values' scale
+        l = fmaf(__uint_as_float((uint32_t)sum) + __uint_as_float((uint32_t)(sum >> 32)), downs[g], l);   // the weights without the values' scale
       }
       tmem_st32(tmem + b * kTile + lanes, pw);       // over the S that this warp has just read
-      alpha *= R == kNone ? 1.0f : pow2i(was - R);
-      if (it > 0 && !wait(pvdone, (it - 1) & 1)) { ok = false; break; }         // O is up to date (waited for tile by tile: a parity tells two phases apart)
-      __syncwarp();
-      tc_fence_after();
+      alpha *= __int_as_float(rest.w);
+      R = rest.z;
+      // Where the unit of O moves, O of the tile in front has to be done.  (S of this tile came after O of tile it - 2: the parity can only be
+      // that of it - 2 or it - 1.)
       if (it > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+        if (!wait(pvdone, (it - 1) & 1)) { ok = false; break; }
+        __syncwarp();
+        tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
@@ -481,10 +535,10 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(pfull);
-      if (d.last) break;
+      if (lane == 0) mbar_arrive(pfull(b));
+      if (rest.y) break;
     }
-    if (ok && tiles > 0) ok = wait(pvdone, it & 1);
+    if (ok && tiles > 0) ok = wait(odone, 0);
     __syncwarp();
     tc_fence_after();
     // a row that sees no key has l = 0: zeros and -inf.  A query that holds an infinity or a NaN has l = NaN and stays NaN.

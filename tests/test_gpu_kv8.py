@@ -203,6 +203,18 @@ def test_sequences_that_share_their_first_pages(cuda, new):
     _check(cache, table, lens, [new] * 3, q, out, lse)
 
 
+@pytest.mark.parametrize("d,ps,news,olds", [(128, 64, [2300, 1500], [0, 300]), (64, 16, [1900, 40, 700], [100, 2000, 0]), (128, 128, [1000] * 12, [200] * 12)])
+def test_long_prompts(cuda, d, ps, news, olds):
+    """More row tiles than fit on the GPU at once, each with many key tiles."""
+    from oxicuda_b200 import _lib as L
+    lens = [n + o for n, o in zip(news, olds)]
+    cache, table = _pages(cuda, lens, ps, 4, d, len(lens))
+    q = _q(cuda, sum(news), 16, d, ps)
+    out, lse = cache.attend(q, torch.tensor(lens, dtype=torch.int32, device=cuda), table, q_starts=_starts(news, cuda), want_lse=True)
+    L.default_handle().check()
+    _check(cache, table, lens, news, q, out, lse)
+
+
 @pytest.mark.parametrize("new,old", [(1, 9000), (2, 9000), (5, 9000), (40, 9000), (130, 6000)])
 def test_long_keys_of_few_rows(cuda, new, old):
     """Keys dealt to the CTAs of a cluster, in every number of them that a batch of this kind meets."""
