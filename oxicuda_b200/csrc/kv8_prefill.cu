@@ -151,11 +151,10 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  // ---- which rows: the longest tiles of a sequence first ----
+  // ---- which rows: the longest tiles of a sequence first, for all heads ----
   const Batch& t = p.t;
-  const int head = blockIdx.y;
+  const int item = (int)(blockIdx.x / split), head = item % t.n_kv_heads, unit = item / t.n_kv_heads;
   const bool tell = head == 0 && part == 0 && warp == 0;
-  const int unit = (int)(blockIdx.x / split);
   if (unit == 0 && tell) for (int b = lane; b < t.seqs; b += 32) rows_of(t, b, true);
   auto count = [&](int b) { return (int)(((int64_t)rows_of(t, b, false).n * p.group + kRows - 1) / kRows); };
   const int2 f = find_unit(t.seqs, unit, count);
@@ -640,9 +639,9 @@ int32_t launch(b2q_handle h, const AttendArgs& p) {
   const int64_t most = (int64_t)p.t.table_width << p.t.page_shift, keys = p.window ? p.window + kTile : most;
   int split = 1;
   while (split < 8 && units * p.t.n_kv_heads * split * 2 <= 2 * (int64_t)h->sm_count && keys >= (int64_t)split * 16 * kTile) split *= 2;
-  if (units * split > 0x7FFFFFFF) B2Q_FAIL(h, B2Q_ERR_INVALID_DIMENSION, "kv8_attention: too many rows");
+  if (units * p.t.n_kv_heads > 0x7FFFFFFF / split) B2Q_FAIL(h, B2Q_ERR_INVALID_DIMENSION, "kv8_attention: too many rows");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(units * split), (unsigned)p.t.n_kv_heads);
+  cfg.gridDim = dim3((unsigned)(units * p.t.n_kv_heads * split));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = h->stream;
