@@ -86,6 +86,13 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 __device__ __forceinline__ uint32_t pack16(uint16_t lo, uint16_t hi) { return (uint32_t)lo | ((uint32_t)hi << 16); }
 
+// one lane of a converged warp, always the same
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 constexpr uint64_t kOne2 = 0x3F8000003F800000ull;   // 1.0f twice
 __device__ __forceinline__ uint64_t dup(float x) { return (uint64_t)__float_as_uint(x) << 32 | __float_as_uint(x); }
 
@@ -137,7 +144,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 
   cg::cluster_group cluster = cg::this_cluster();
   const int split = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     s_abort = 0;
     for (int s = 0; s < kKStages; ++s) { mbar_init(kfull(s), 1); mbar_init(kempty(s), 1); }
@@ -196,7 +203,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   tc_fence_after();
   // only now may the next kernel start launching: it may take TMEM of its own before it waits for this one
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const uint32_t tmem = s_tmem_base, tmem_o = tmem + 2 * kTile;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem_base, 0), tmem_o = tmem + 2 * kTile;
   volatile int* abort_flag = &s_abort;
   auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, abort_flag, kWaitLimitNs, 1); };
 
@@ -345,14 +352,17 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       }
     } else if (warp == 1) {
       // ---------------- MMA issuer: S of the next tile goes out before O of this one ----------------
-      if (lane == 0) {
-        const uint32_t id_s = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);                // E4M3 x E4M3, f32 sums
-        const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);      // f16 x f16; V: channels contiguous
-        bool ok = wait(qready, 0);
-        auto scores = [&](int it) {
-          const int s = it % kKStages, b = it & 1;
-          if (!wait(kfull(s), (it / kKStages) & 1)) return false;
-          tc_fence_after();
+      // The warp stays together and elects a lane for each group of products: descriptors then live in uniform registers.  One lane alone
+      // in its branch moved each operand there, product by product, and that chain bounded the kernel (5 % of its time).
+      const uint32_t id_s = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);                // E4M3 x E4M3, f32 sums
+      const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);      // f16 x f16; V: channels contiguous
+      auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
+      bool ok = all_wait(qready, 0);
+      auto scores = [&](int it) {
+        const int s = it % kKStages, b = it & 1;
+        if (!all_wait(kfull(s), (it / kKStages) & 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
           const uint32_t kt = k_at + s * C::kTileBytes;
 #pragma unroll
           for (int term = 0; term < 2; ++term) {
@@ -363,16 +373,19 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           }
           tc_commit(kempty(s));
           tc_commit(sfull(b));
-          return true;
-        };
-        ok = ok && scores(0);
-        for (int it = 0; ok; ++it) {
-          const int last = s_info[it % kInfo].last;   // written before the tile's copies were issued, which scores(it) waited for
-          // S of tile it + 1 overwrites S and P of tile it - 1: their product has to be done
-          if (!last && !(ok = (it == 0 || wait(pvdone, (it - 1) & 1)) && scores(it + 1))) break;
-          const int b = it & 1;
-          if (!wait(wfull(b), (it >> 1) & 1) || !wait(pfull(b), (it >> 1) & 1)) { ok = false; break; }
-          tc_fence_after();
+        }
+        __syncwarp();
+        return true;
+      };
+      ok = ok && scores(0);
+      for (int it = 0; ok; ++it) {
+        const int last = __shfl_sync(0xffffffffu, s_info[it % kInfo].last, 0);   // written before the tile's copies were issued, which scores(it) waited for
+        // S of tile it + 1 overwrites S and P of tile it - 1: their product has to be done
+        if (!last && !(ok = (it == 0 || all_wait(pvdone, (it - 1) & 1)) && scores(it + 1))) break;
+        const int b = it & 1;
+        if (!all_wait(wfull(b), (it >> 1) & 1) || !all_wait(pfull(b), (it >> 1) & 1)) { ok = false; break; }
+        tc_fence_after();
+        if (elect_one()) {
           const uint32_t vt = w_at + b * C::kV16;
           // 16 keys a step: two groups of 8 rows of 128 bytes; blocks of 64 channels lie 64 rows apart (leading byte offset)
 #pragma unroll
@@ -382,15 +395,18 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           }
           tc_commit(wempty(b));
           tc_commit(pvdone);
-          if (last) { tc_commit(odone); break; }
+          if (last) tc_commit(odone);
         }
-        if (!ok) {
-          tc_commit(drain);
-          const uint64_t t0 = globaltimer_ns();
-          while (!mbar_try_wait(drain, 0))
-            if (globaltimer_ns() - t0 > 100000000ull) break;
-        }
+        __syncwarp();
+        if (last) break;
       }
+      if (!ok && elect_one()) {
+        tc_commit(drain);
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(drain, 0))
+          if (globaltimer_ns() - t0 > 100000000ull) break;
+      }
+      __syncwarp();
     } else {
       // ---------------- values to f16, 64 threads: 16 channels of a key at a time ----------------
       // a thread keeps its unit u of 16 channels and its key modulo KEYS (a multiple of 8), so the swizzles are fixed
