@@ -133,7 +133,7 @@ gemm_block128_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // the same in all lanes, and known to be
   const uint32_t rank = cluster_ctarank();              // 0 = leader (issues the MMAs), 1 = peer
   const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
   const int total = p.tiles_m * p.tiles_n, num_kb = p.kb;
@@ -155,7 +155,7 @@ gemm_block128_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
   __syncthreads();
   cluster_sync_all();                                   // both CTAs' barriers exist before anyone signals across
   tc_fence_after();
-  const uint32_t tmem_base = s_tmem_base;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, s_tmem_base, 0);
   volatile int* abort_flag = &s_abort;
   b2q_pdl_entry();                                      // everything above may overlap the previous kernel of the stream
 
@@ -186,24 +186,29 @@ gemm_block128_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
       }
     } else if (warp == 1) {
       // ---------------- MMA issuer (leader CTA only): one accumulator per block of K ----------------
-      if (lane == 0 && rank == 0) {
+      // The warp stays together and elects a lane for the products of a block: descriptors then live in uniform registers.
+      if (rank == 0) {
         uint32_t it = 0;
         bool ok = true;
         for (int u = pair; u < total && ok; u += num_pairs) {
           for (int kb = 0; kb < num_kb; ++kb, ++it) {
             const int s = it % kStages, b = it % kBuf;
-            if (!mbar_wait(tempty_bar(b), ((it / kBuf) & 1) ^ 1, abort_flag) || !mbar_wait(full_bar(s), (it / kStages) & 1, abort_flag)) { ok = false; break; }
+            ok = __all_sync(0xffffffffu, mbar_wait(tempty_bar(b), ((it / kBuf) & 1) ^ 1, abort_flag) && mbar_wait(full_bar(s), (it / kStages) & 1, abort_flag));
+            if (!ok) break;
             tc_fence_after();
-            const uint32_t sa = base + s * C::kStageBytes;
-            const uint64_t adesc = make_desc_sw128(sa), bdesc = make_desc_sw128(sa + C::kBytesA);
+            if (elect_one()) {
+              const uint32_t sa = base + s * C::kStageBytes;
+              const uint64_t adesc = make_desc_sw128(sa), bdesc = make_desc_sw128(sa + C::kBytesA);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)                   // K advance inside the swizzle atom: +32 bytes
-              umma_pair(tmem_base + b * BN, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), p.idesc, (uint32_t)(k != 0));
-            tc_commit_pair(empty_bar(s));
-            tc_commit_pair(tfull_bar(b));
+              for (int k = 0; k < 4; ++k)                   // K advance inside the swizzle atom: +32 bytes
+                umma_pair(tmem_base + b * BN, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), p.idesc, (uint32_t)(k != 0));
+              tc_commit_pair(empty_bar(s));
+              tc_commit_pair(tfull_bar(b));
+            }
+            __syncwarp();
           }
         }
-        if (!ok) {
+        if (!ok && elect_one()) {
           tc_commit(drain_bar);
           const uint64_t t0 = globaltimer_ns();
           while (!mbar_try_wait(drain_bar, 0))

@@ -75,7 +75,7 @@ gemm_block128_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
 
   cg::cluster_group cluster = cg::this_cluster();
   const int split = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // the same in all lanes, and known to be
   const int tile = (int)(blockIdx.x / split);
   const int k_begin = (int)((int64_t)p.kb * part / split), k_end = (int)((int64_t)p.kb * (part + 1) / split), total = k_end - k_begin;
 
@@ -98,7 +98,7 @@ gemm_block128_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = s_tmem_base;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, s_tmem_base, 0);
   volatile int* abort_flag = &s_abort;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -129,13 +129,14 @@ gemm_block128_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
       }
     }
   } else if (warp == 1) {
-    // ---------------- MMA issuer: one accumulator per block of K ----------------
-    if (lane == 0) {
-      bool ok = true;
-      for (int it = 0; it < total; ++it) {
-        const int s = it % kStages, b = it % kBuf;
-        if (!mbar_wait(tempty_bar(b), ((it / kBuf) & 1) ^ 1, abort_flag) || !mbar_wait(full_bar(s), (it / kStages) & 1, abort_flag)) { ok = false; break; }
-        tc_fence_after();
+    // ---------------- MMA issuer: one accumulator per block of K; the warp stays together and elects a lane (descriptors in uniform registers) ----------------
+    bool ok = true;
+    for (int it = 0; it < total; ++it) {
+      const int s = it % kStages, b = it % kBuf;
+      ok = __all_sync(0xffffffffu, mbar_wait(tempty_bar(b), ((it / kBuf) & 1) ^ 1, abort_flag) && mbar_wait(full_bar(s), (it / kStages) & 1, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
         const uint32_t sw = base + s * C::kStageBytes;
         const uint64_t adesc = make_desc_sw128(sw), bdesc = make_desc_sw128(sw + C::kBytesW);
 #pragma unroll
@@ -144,12 +145,13 @@ gemm_block128_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
         tc_commit(empty_bar(s));
         tc_commit(tfull_bar(b));
       }
-      if (!ok) {
-        tc_commit(drain_bar);
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(drain_bar, 0))
-          if (globaltimer_ns() - t0 > 100000000ull) break;
-      }
+      __syncwarp();
+    }
+    if (!ok && elect_one()) {
+      tc_commit(drain_bar);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(drain_bar, 0))
+        if (globaltimer_ns() - t0 > 100000000ull) break;
     }
   } else if (warp < 4) {
     // ---------------- scales: scale_a * scale_w of each token, four blocks of K at a time ----------------

@@ -86,13 +86,6 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 __device__ __forceinline__ uint32_t pack16(uint16_t lo, uint16_t hi) { return (uint32_t)lo | ((uint32_t)hi << 16); }
 
-// one lane of a converged warp, always the same
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
-  return p != 0;
-}
-
 constexpr uint64_t kOne2 = 0x3F8000003F800000ull;   // 1.0f twice
 __device__ __forceinline__ uint64_t dup(float x) { return (uint64_t)__float_as_uint(x) << 32 | __float_as_uint(x); }
 
