@@ -46,39 +46,43 @@ __device__ __forceinline__ int page_of(const Batch& t, int b, int index, bool te
   return pg;
 }
 
-// Finds the unit'th item of a list in which sequence b has count(b) items, by a whole warp: {b, index within b}, b = -1 past the end.
+// Finds the unit'th item of a list in which sequence b has count(b) items, by a whole warp: {b, index within b, count(b)}, b = -1 past the
+// end.  All counts of a possible batch fit 31 bits together; those of an impossible one may wrap, so the index is checked against its count.
+struct Found { int b, index, count; };
 template <typename F>
-__device__ __forceinline__ int2 find_unit(int seqs, int64_t unit, F count) {
+__device__ __forceinline__ Found find_unit(int seqs, int unit, F count) {
   const int lane = threadIdx.x & 31;
   for (int b0 = 0; b0 < seqs; b0 += 32) {
     const int c = b0 + lane < seqs ? count(b0 + lane) : 0;
-    int64_t s = c;
+    int s = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, s, o);
+      const int up = __shfl_up_sync(0xffffffffu, s, o);
       if (lane >= o) s += up;
     }
-    const int64_t total = __shfl_sync(0xffffffffu, s, 31);
-    if (unit < total) {
-      const unsigned hit = __ballot_sync(0xffffffffu, s > unit);
-      const int src = __ffs(hit) - 1;
-      const int64_t before = __shfl_sync(0xffffffffu, s - c, src);
-      return make_int2(b0 + src, (int)(unit - before));
+    const unsigned hit = __ballot_sync(0xffffffffu, s > unit);
+    if (hit) {
+      const int src = __ffs(hit) - 1, at = __shfl_sync(0xffffffffu, unit - (s - c), src), n = __shfl_sync(0xffffffffu, c, src);
+      return (unsigned)at < (unsigned)n ? Found{b0 + src, at, n} : Found{-1, 0, 0};
     }
-    unit -= total;
+    unit -= __shfl_sync(0xffffffffu, s, 31);
   }
-  return make_int2(-1, 0);
+  return Found{-1, 0, 0};
 }
 
 struct AttendArgs {
   Batch t;
   const __nv_bfloat16* q; int64_t ld_q;
   const uint8_t* k; const uint8_t* v; const uint8_t* ks; const uint8_t* vs;
-  int group;                                     // query heads per kv head
+  int group;                                     // query heads per kv head, at most 2^20
+  float per_group;                               // 1 / group
   int window;                                    // 0: none
   float scale;                                   // softmax scale * log2(e)
   __nv_bfloat16* out; float* lse;                // [tokens][heads][head_dim], [tokens][heads]
 };
+
+// x / group and x % group for 0 <= x < 2^21: (x + 1/2) / group lies 1 / (2 group) off an integer at least, which the roundings do not reach
+__device__ __forceinline__ int div_group(const AttendArgs& p, int x) { return (int)(((float)x + 0.5f) * p.per_group); }
 
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(min(127, max(-126, e)) + 127) << 23); }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }

@@ -83,21 +83,21 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(const AppendArgs p) {
   if (item >= (int64_t)p.units * per) return;
   const int unit = (int)(item / per), head = (int)(item % per) >> 1, kv = (int)(item & 1);
   const bool tell = head == 0 && kv == 0 && (W == 1 || warp == 0);
-  int2 f;
-  if (SINGLE) f = make_int2(unit, 0);
+  Found f;
+  if (SINGLE) f = Found{unit, 0, 1};
   else {
     if (unit == 0 && tell) for (int b = lane; b < t.seqs; b += 32) rows_of(t, b, true);
     f = find_unit(t.seqs, unit, [&](int b) {
       const Rows r = rows_of(t, b, false);
       return r.n > 0 ? ((r.len - 1) >> t.page_shift) - ((r.len - r.n) >> t.page_shift) + 1 : 0;
     });
-    if (f.x < 0) return;
+    if (f.b < 0) return;
   }
-  const Rows r = rows_of(t, f.x, SINGLE && tell && lane == 0);
+  const Rows r = rows_of(t, f.b, SINGLE && tell && lane == 0);
   if (r.n == 0) return;
   const int first = r.len - r.n;                                        // position of the first new token
-  const int index = (first >> t.page_shift) + f.y;
-  const int pg = page_of(t, f.x, index, tell && lane == 0);
+  const int index = (first >> t.page_shift) + f.index;
+  const int pg = page_of(t, f.b, index, tell && lane == 0);
   if (pg < 0) return;
   const int base = index << t.page_shift;
   const int lo = max(first, base), n = min(r.len, base + ps) - lo;      // first position and number of rows that this page receives

@@ -120,17 +120,17 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const int unit = (int)(blockIdx.x / split);
   const bool tell = head == 0 && part == 0 && warp == 0;
 
-  int2 f;
+  Found f;
   if (t.q_starts == nullptr) {
     const int per = (p.group + kRows - 1) / kRows;
-    f = make_int2(unit / per, unit % per);
+    f = Found{unit / per, unit % per, per};
   } else {
     if (unit == 0 && tell) for (int b = lane; b < t.seqs; b += 32) rows_of(t, b, true);
     f = find_unit(t.seqs, unit, [&](int b) { return (rows_of(t, b, false).n * p.group + kRows - 1) / kRows; });
-    if (f.x < 0) return;                          // the whole cluster leaves: every CTA of it has the same unit
+    if (f.b < 0) return;                          // the whole cluster leaves: every CTA of it has the same unit
   }
-  const Rows r = rows_of(t, f.x, tell && t.q_starts == nullptr && lane == 0);
-  const int row0 = f.y * kRows, valid = min(kRows, r.n * p.group - row0);   // rows of all sequences fit 31 bits; <= 0: an impossible sequence
+  const Rows r = rows_of(t, f.b, tell && t.q_starts == nullptr && lane == 0);
+  const int row0 = f.index * kRows, valid = min(kRows, r.n * p.group - row0);   // rows of all sequences fit 31 bits; <= 0: an impossible sequence
   if (valid <= 0) return;                         // its rows stay as they are
   const int token0 = row0 / p.group, head0 = row0 - token0 * p.group;       // of the first row, within the sequence and the group
   const int first_pos = r.len - r.n + token0, last_pos = first_pos + (head0 + valid - 1) / p.group;
@@ -164,7 +164,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int j = j0 + rows_each * e;
-        pg[e] = e < subs && i0 + lane < mine && j < key_end && (j | (rows_each - 1)) >= key_low ? page_of(t, f.x, j >> t.page_shift, head == 0) : -1;
+        pg[e] = e < subs && i0 + lane < mine && j < key_end && (j | (rows_each - 1)) >= key_low ? page_of(t, f.b, j >> t.page_shift, head == 0) : -1;
       }
     };
     auto scales = [&] {
@@ -603,7 +603,9 @@ extern "C" int32_t b2q_kv8_attention_bf16(b2q_handle h, const void* q, int64_t l
   if (window < 0) B2Q_FAIL(h, B2Q_ERR_INVALID_ARGUMENT, "kv8_attention: window %lld is negative", (long long)window);
   p.q = static_cast<const __nv_bfloat16*>(q); p.ld_q = ld_q;
   p.k = k_codes; p.v = v_codes; p.ks = k_scales; p.vs = v_scales;
+  if (n_heads / n_kv_heads > 1 << 20) B2Q_FAIL(h, B2Q_ERR_INVALID_DIMENSION, "kv8_attention: %lld query heads are too many", (long long)n_heads);
   p.group = (int)(n_heads / n_kv_heads);
+  p.per_group = 1.0f / (float)p.group;
   const int64_t most = table_width * page_size;                        // keys that a sequence can have
   p.window = window > 0 && window < most ? (int)window : 0;
   p.scale = scale * 1.4426950408889634f;

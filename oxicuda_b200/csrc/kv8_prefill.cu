@@ -42,6 +42,7 @@ constexpr int kRoom = 2;                         // R is set that far above a sc
 constexpr int kNone = -1000;
 constexpr float kSlack = 6.0f;                   // 2^(8 + 6) is well inside f16
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
+constexpr int kGridY = 32768;                    // row tiles: blockIdx.y, and z beyond that
 
 template <int D> struct Cfg {
   static constexpr int kQ = 2 * kRows * D;       // both terms
@@ -85,6 +86,8 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ uint32_t pack16(uint16_t lo, uint16_t hi) { return (uint32_t)lo | ((uint32_t)hi << 16); }
+
+__device__ __forceinline__ uint32_t cluster_id_x() { uint32_t r; asm("mov.u32 %0, %clusterid.x;" : "=r"(r)); return r; }
 
 constexpr uint64_t kOne2 = 0x3F8000003F800000ull;   // 1.0f twice
 __device__ __forceinline__ uint64_t dup(float x) { return (uint64_t)__float_as_uint(x) << 32 | __float_as_uint(x); }
@@ -153,17 +156,15 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 
   // ---- which rows: the longest tiles of a sequence first, for all heads ----
   const Batch& t = p.t;
-  const int item = (int)(blockIdx.x / split), head = item % t.n_kv_heads, unit = item / t.n_kv_heads;
+  const int head = (int)cluster_id_x(), unit = (int)(blockIdx.y + kGridY * blockIdx.z);
   const bool tell = head == 0 && part == 0 && warp == 0;
   if (unit == 0 && tell) for (int b = lane; b < t.seqs; b += 32) rows_of(t, b, true);
-  auto count = [&](int b) { return (int)(((int64_t)rows_of(t, b, false).n * p.group + kRows - 1) / kRows); };
-  const int2 f = find_unit(t.seqs, unit, count);
-  if (f.x < 0) return;                            // the whole cluster leaves, before it holds TMEM
-  const Rows r = rows_of(t, f.x, false);
-  const int64_t row0 = (int64_t)(count(f.x) - 1 - f.y) * kRows;
-  const int valid = (int)min((int64_t)kRows, (int64_t)r.n * p.group - row0);
-  const int token0 = (int)(row0 / p.group), head0 = (int)(row0 - (int64_t)token0 * p.group);   // of the tile's first row, within the sequence and the group
-  const int first_pos = r.len - r.n + token0, last_pos = first_pos + (head0 + valid - 1) / p.group;
+  const Found f = find_unit(t.seqs, unit, [&](int b) { return (rows_of(t, b, false).n * p.group + kRows - 1) / kRows; });
+  if (f.b < 0) return;                            // the whole cluster leaves, before it holds TMEM
+  const Rows r = rows_of(t, f.b, false);          // rows of all sequences fit 31 bits
+  const int row0 = (f.count - 1 - f.index) * kRows, valid = min(kRows, r.n * p.group - row0);
+  const int token0 = row0 / p.group, head0 = row0 - token0 * p.group;        // of the tile's first row, within the sequence and the group
+  const int first_pos = r.len - r.n + token0, last_pos = first_pos + div_group(p, head0 + valid - 1);
   const int key_end = last_pos + 1;
   // the first key that a row sees; the first tile may begin before it, with pages that its owner has given up and that are not looked up
   const int key_low = p.window > 0 ? max(0, first_pos - p.window + 1) : 0, key_begin = key_low & ~(kTile - 1);
@@ -180,8 +181,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   auto qrow_of = [&](int i, int j) { return RPW * (warp - 1 + 7 * i) + j; };  // row j of turn i
   if (warp > 0) {
     const int mine = qrow_of(lane / RPW, lane % RPW);
-    const int hr = head0 + (mine < valid ? mine : 0);                         // rows behind the last one: the first row's
-    const __nv_bfloat16* const at = p.q + (int64_t)(r.r0 + token0 + hr / p.group) * p.ld_q + (int64_t)(head * p.group + hr % p.group) * D;
+    const int hr = head0 + (mine < valid ? mine : 0), tk = div_group(p, hr);   // rows behind the last one: the first row's
+    const __nv_bfloat16* const at = p.q + (int64_t)(r.r0 + token0 + tk) * p.ld_q + (int64_t)(head * p.group + hr - tk * p.group) * D;
 #pragma unroll 1
     for (int i = 0; i < QI; ++i) {
       const int rr = qrow_of(i, lane / LPR);
@@ -255,7 +256,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           pg[e] = -1; info[e] = 0;
           const int j = j0 + rows_each * e;
           if (e < subs && i0 + lane < tiles && j < key_end && (j | (rows_each - 1)) >= key_low) {
-            pg[e] = page_of(t, f.x, j >> t.page_shift, head == 0);
+            pg[e] = page_of(t, f.b, j >> t.page_shift, head == 0);
             if (pg[e] >= 0)
               info[e] = kThere | (uint32_t)p.ks[(int64_t)pg[e] * t.n_kv_heads + head] | ((uint32_t)p.vs[(int64_t)pg[e] * t.n_kv_heads + head] << 8);
           }
@@ -442,7 +443,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     const int quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const bool live = row < valid;
-    const int token = live ? token0 + (head0 + row) / p.group : 0, qhead = head * p.group + (live ? (head0 + row) % p.group : 0);
+    const int tk = live ? div_group(p, head0 + row) : 0, token = live ? token0 + tk : 0, qhead = head * p.group + (live ? head0 + row - tk * p.group : 0);
     const int pos = live ? r.len - r.n + token : -1;
     if (!wait(qready, 0)) tiles = -1;               // only if another warp has given up
     const float qf = s_m[row];
@@ -610,8 +611,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(smem + row * (D * 4) + ((u ^ (row & 7)) << 4), c));
         acc.x += fo * x.x; acc.y += fo * x.y; acc.z += fo * x.z; acc.w += fo * x.w;
       }
-      const int tk = token0 + (head0 + row) / p.group, hd = head * p.group + (head0 + row) % p.group;
-      const int64_t orow = (int64_t)(r.r0 + tk) * (t.n_kv_heads * p.group) + hd;
+      const int tk = div_group(p, head0 + row), hd = head * p.group + head0 + row - tk * p.group;
+      const int64_t orow = (int64_t)(r.r0 + token0 + tk) * (t.n_kv_heads * p.group) + hd;
       const float inv = ll == 0.0f ? 0.0f : __frcp_rn(ll), up = rr == kNone ? 0.0f : pow2i(rr - 8);
       const __nv_bfloat162 y0 = __floats2bfloat162_rn(acc.x * inv * up, acc.y * inv * up), y1 = __floats2bfloat162_rn(acc.z * inv * up, acc.w * inv * up);
       uint2 pk;
@@ -648,9 +649,8 @@ int32_t launch(b2q_handle h, const AttendArgs& p) {
   const int64_t most = (int64_t)p.t.table_width << p.t.page_shift, keys = p.window ? p.window + kTile : most;
   int split = 1;
   while (split < 8 && units * p.t.n_kv_heads * split * 2 <= 2 * (int64_t)h->sm_count && keys >= (int64_t)split * 16 * kTile) split *= 2;
-  if (units * p.t.n_kv_heads > 0x7FFFFFFF / split) B2Q_FAIL(h, B2Q_ERR_INVALID_DIMENSION, "kv8_attention: too many rows");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(units * p.t.n_kv_heads * split));
+  cfg.gridDim = dim3((unsigned)(p.t.n_kv_heads * split), (unsigned)(units < kGridY ? units : kGridY), (unsigned)ceil_div64(units, kGridY));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = h->stream;
