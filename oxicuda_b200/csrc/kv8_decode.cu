@@ -116,7 +116,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   cg::cluster_group cluster = cg::this_cluster();
   const int split = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const Batch& t = p.t;
-  const int head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lr = lane >> 2, tq = lane & 3;
+  const int head = blockIdx.y, warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, lr = lane >> 2, tq = lane & 3;
   const int unit = (int)(blockIdx.x / split);
   const bool tell = head == 0 && part == 0 && warp == 0;
 
@@ -173,7 +173,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         info[e] = pg[e] < 0 ? 0u : 0x80000000u | (uint32_t)p.ks[(int64_t)pg[e] * t.n_kv_heads + head] | ((uint32_t)p.vs[(int64_t)pg[e] * t.n_kv_heads + head] << 8);
     };
     // A lane leaves the lines of its tile's pages (the maps see lines of 128 bytes: one token of 128 channels, or two of 64; -1: no page) and
-    // the scales in shared memory; lane 0 alone issues, without a step of the other lanes in between.
+    // the scales in shared memory.  The warp stays together and elects a lane to issue, so that a copy's operands live in uniform registers: with
+    // lane 0 alone in a branch, 32 x 8200 keys in pages of 16 (eight copies to a tile) took 113 us instead of 94.
     auto leave = [&](int i0) {
       const int in_page = (key_begin + kTile * (part + split * (i0 + lane))) & ((1 << t.page_shift) - 1);   // 0 but for pages of 128
       int line[4];
@@ -212,20 +213,22 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     for (int i0 = 0; i0 < mine && ok; i0 += 32) {
       s_words[lane] = words();
       __syncwarp();
-      if (i0 + 32 < mine) { pages(i0 + 32); scales(); }                // in flight while lane 0 issues
-      if (lane == 0) {
-        const int n = min(32, mine - i0);
-        for (int i = i0 ? 0 : lead_in; i < n; ++i) {
-          const int st = (i0 + i) % G::kStages;
-          const int4 ln = s_line[i];
-          const uint4 w = s_words[i];
-          if (!mbar_wait_bounded(empty_bar(st), (((i0 + i) / G::kStages) & 1) ^ 1, abort_flag, kWaitLimitNs, 1)) { ok = false; break; }
-          copy(st, ln);
+      if (i0 + 32 < mine) { pages(i0 + 32); scales(); }                // in flight while the copies are issued
+      const int n = min(32, mine - i0);
+      for (int i = i0 ? 0 : lead_in; i < n; ++i) {
+        const int st = (i0 + i) % G::kStages;
+        const int4 ln = s_line[i];
+        const uint4 w = s_words[i];
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(empty_bar(st), (((i0 + i) / G::kStages) & 1) ^ 1, abort_flag, kWaitLimitNs, 1));
+        if (!ok) break;
+        const int4 same = make_int4(__shfl_sync(0xffffffffu, ln.x, 0), __shfl_sync(0xffffffffu, ln.y, 0), __shfl_sync(0xffffffffu, ln.z, 0), __shfl_sync(0xffffffffu, ln.w, 0));
+        if (elect_one()) {
+          copy(st, same);
           s_info[st] = w;
           mbar_arrive(full_bar(st));
         }
+        __syncwarp();
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
       leave(i0 + 32);
     }
     if (!ok && lane == 0) {                      // give copies in flight time to land before shared memory is released
