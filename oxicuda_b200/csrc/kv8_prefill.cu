@@ -114,7 +114,9 @@ __device__ __forceinline__ void landed(uint32_t (&r)[64]) {
     asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
-template <int D>
+// SUBS: pages that a tile of keys spans (1: pages of 64 and 128), known at compile time: the producer's share of a tile is then a third shorter,
+// and that was on the critical path (2 x 3900 tokens 308 -> 289 us)
+template <int D, int SUBS>
 __global__ void __launch_bounds__(kThreads, 2)
 kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttendArgs p) {
   using C = Cfg<D>;
@@ -171,12 +173,12 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   const int all = (key_end - key_begin + kTile - 1) / kTile;
   int tiles = (all - part + split - 1) / split;   // tiles part, part + split, ..
 
-  // ---------------- the query rows, by warps 1 .. 7: D / 8 lanes to a row, 8 channels each, so that a warp reads whole rows ----------------
+  // ---------------- the query rows, by warps 1 .. 7: D / 16 lanes to a row, 16 channels (16 bytes of codes) each ----------------
   // They come in through the space of the f16 value tiles (free until the first of those is made), and a short loop turns them: unrolled
   // over registers the same work was 13 KB of code that every CTA fetched once, 7 us.
-  constexpr int LPR = D / 8, RPW = 32 / LPR, QI = (kRows / RPW + 6) / 7;      // lanes to a row, rows at once, turns of a warp
+  constexpr int LPR = D / 16, RPW = 32 / LPR, QI = (kRows / RPW + 6) / 7;     // lanes to a row, rows at once, turns of a warp
   static_assert(QI * RPW <= 32, "a lane holds the address of each row");
-  const int qc = lane % LPR;                                                  // 16 bytes of bf16 = half a 16-byte unit of codes
+  const int qc = lane % LPR;
   uint8_t* const raw = smem + (w_at - base);
   auto qrow_of = [&](int i, int j) { return RPW * (warp - 1 + 7 * i) + j; };  // row j of turn i
   if (warp > 0) {
@@ -186,8 +188,12 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 #pragma unroll 1
     for (int i = 0; i < QI; ++i) {
       const int rr = qrow_of(i, lane / LPR);
-      const unsigned long long from = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), i * RPW + lane / LPR) + 16 * qc;
-      if (rr < kRows) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(raw + rr * (2 * D) + 16 * qc)), "l"(from) : "memory");
+      const unsigned long long from = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), i * RPW + lane / LPR) + 32 * qc;
+      const uint32_t to = smem_u32(raw + rr * (2 * D) + 32 * qc);
+      if (rr < kRows) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 16), "l"(from + 16) : "memory");
+      }
     }
   }
 
@@ -207,30 +213,35 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     __syncwarp();
 #pragma unroll 1
     for (int i = 0; i < QI; ++i) {
-      const int rr = qrow_of(i, lane / LPR), from = min(rr, kRows - 1);
-      const uint4 w = *reinterpret_cast<const uint4*>(raw + from * (2 * D) + 16 * qc);
-      const __nv_bfloat162* const q2 = reinterpret_cast<const __nv_bfloat162*>(&w);
+      const int rr = qrow_of(i, lane / LPR);
+      const uint4* const from = reinterpret_cast<const uint4*>(raw + min(rr, kRows - 1) * (2 * D) + 32 * qc);
+      const uint4 w[2] = {from[0], from[1]};
+      const __nv_bfloat162* const q2 = reinterpret_cast<const __nv_bfloat162*>(w);
       // the largest of the row, a NaN if it holds one
-      __nv_bfloat162 top = __hmax2_nan(__hmax2_nan(__habs2(q2[0]), __habs2(q2[1])), __hmax2_nan(__habs2(q2[2]), __habs2(q2[3])));
+      __nv_bfloat162 top = __habs2(q2[0]);
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top = __hmax2_nan(top, __habs2(q2[j]));
 #pragma unroll
       for (int o = LPR / 2; o > 0; o >>= 1) top = __hmax2_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
       const float amax = __bfloat162float(__hmax_nan(top.x, top.y));
       const uint32_t u = __float_as_uint(amax);
       const int e = max(-119, (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0));
       const float inv = sign * pow2i(-e);
-      uint16_t h[4], l[4];
+      uint32_t h[4], l[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {                                            // exact in f16 down to 2^-24
-        const float2 x = __bfloat1622float2(q2[j]);
-        split_f16(pack_f16(x.x * inv, x.y * inv), h[j], l[j]);
+        uint16_t ha, la, hb, lb;
+        const float2 x = __bfloat1622float2(q2[2 * j]), y = __bfloat1622float2(q2[2 * j + 1]);
+        split_f16(pack_f16(x.x * inv, x.y * inv), ha, la);
+        split_f16(pack_f16(y.x * inv, y.y * inv), hb, lb);
+        h[j] = pack16(ha, hb);
+        l[j] = pack16(la, lb);
       }
       if (rr < kRows) {
         // rows of 128 bytes, 128-byte swizzle; 64 channels: both terms share a row
         uint8_t* const qrow = smem + rr * 128;
-        const int unit16 = qc >> 1, in16 = (qc & 1) * 8;
-        *reinterpret_cast<uint2*>(qrow + ((unit16 ^ (rr & 7)) << 4) + in16) = make_uint2(pack16(h[0], h[1]), pack16(h[2], h[3]));
-        *reinterpret_cast<uint2*>(qrow + (D == 128 ? kRows * 128 + ((unit16 ^ (rr & 7)) << 4) : ((unit16 + 4) ^ (rr & 7)) << 4) + in16) =
-            make_uint2(pack16(l[0], l[1]), pack16(l[2], l[3]));
+        *reinterpret_cast<uint4*>(qrow + ((qc ^ (rr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(qrow + (D == 128 ? kRows * 128 + ((qc ^ (rr & 7)) << 4) : ((qc + 4) ^ (rr & 7)) << 4)) = make_uint4(l[0], l[1], l[2], l[3]);
         // a query with an infinity or a NaN: NaN throughout
         if (qc == 0) s_m[rr] = amax < INFINITY ? fabsf(p.scale) * pow2i(e) : __uint_as_float(0x7FC00000u);
       }
@@ -246,16 +257,16 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       // a CTA of the cluster beyond the last tile: it only joins
     } else if (warp == 0) {
       // ---------------- producer: pages and scales of 32 tiles at a time (a tile to a lane), fetched while the 32 before are issued ----------------
-      const int subs = t.page_shift >= 6 ? 1 : kTile >> t.page_shift, rows_each = kTile / subs;
-      int pg[4];
-      uint32_t info[4];
+      constexpr int rows_each = kTile / SUBS;
+      int pg[SUBS];
+      uint32_t info[SUBS];
       auto fetch = [&](int i0) {
         const int j0 = key_begin + kTile * (part + split * (i0 + lane));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < SUBS; ++e) {
           pg[e] = -1; info[e] = 0;
           const int j = j0 + rows_each * e;
-          if (e < subs && i0 + lane < tiles && j < key_end && (j | (rows_each - 1)) >= key_low) {
+          if (i0 + lane < tiles && j < key_end && (j | (rows_each - 1)) >= key_low) {
             pg[e] = page_of(t, f.b, j >> t.page_shift, head == 0);
             if (pg[e] >= 0)
               info[e] = kThere | (uint32_t)p.ks[(int64_t)pg[e] * t.n_kv_heads + head] | ((uint32_t)p.vs[(int64_t)pg[e] * t.n_kv_heads + head] << 8);
@@ -266,76 +277,74 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       int R = kNone, it = 0;                        // tiles issued: a tile is walked once per group of pages whose value scales are alike
       fetch(0);
       for (int i0 = 0; i0 < tiles && ok; i0 += 32) {
-        int cp[4];
-        uint32_t ci[4];
+        int cp[SUBS];
+        uint32_t ci[SUBS];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { cp[e] = pg[e]; ci[e] = info[e]; }
+        for (int e = 0; e < SUBS; ++e) { cp[e] = pg[e]; ci[e] = info[e]; }
         if (i0 + 32 < tiles) fetch(i0 + 32);
         const int n = min(32, tiles - i0);
         for (int i = 0; i < n && ok; ++i) {
-          const int j = key_begin + kTile * (part + split * (i0 + i));
-          int p4[4];
-          uint32_t f4[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (e >= subs) { p4[e] = -1; f4[e] = 0; continue; }
-            p4[e] = __shfl_sync(0xffffffffu, cp[e], i); f4[e] = __shfl_sync(0xffffffffu, ci[e], i);
-          }
+          const int j = key_begin + kTile * (part + split * (i0 + i)), in_page = j & ((1 << t.page_shift) - 1);   // in_page: 0 but for pages of 128
+          int line[SUBS], there = 0;                // first row of the page in the map, or -1
+          uint32_t fl[SUBS];
           unsigned rem = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) rem |= p4[e] >= 0 ? 1u << e : 0u;
+          for (int e = 0; e < SUBS; ++e) {
+            const int pe = __shfl_sync(0xffffffffu, cp[e], i);
+            fl[e] = __shfl_sync(0xffffffffu, ci[e], i);
+            line[e] = pe >= 0 ? ((pe * t.n_kv_heads + head) << t.page_shift) + in_page : -1;
+            there += pe >= 0;
+            rem |= pe >= 0 ? 1u << e : 0u;
+          }
           bool once = true;                         // a tile without any page is walked too: its rows see none of it
           while ((rem || once) && ok) {
             once = false;
             int lead = kNone;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) if (rem >> e & 1) lead = max(lead, (int)(f4[e] >> 8 & 0xFF) - 127);
             unsigned take = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) take |= (rem >> e & 1) && (int)(f4[e] >> 8 & 0xFF) - 127 >= lead - kSpan ? 1u << e : 0u;
+            for (int e = 0; e < SUBS; ++e) if (rem >> e & 1) lead = max(lead, (int)(fl[e] >> 8 & 0xFF) - 127);
+#pragma unroll
+            for (int e = 0; e < SUBS; ++e) take |= (rem >> e & 1) && (int)(fl[e] >> 8 & 0xFF) - 127 >= lead - kSpan ? 1u << e : 0u;
             rem &= ~take;
-            const int s = it % kKStages, v = it % kVStages;
-            if (lane == 0) {
-              ok = wait(kempty(s), ((it / kKStages) & 1) ^ 1);
-              if (ok) {
-                const int was = R == kNone ? lead + kRoom : R;
-                R = lead == kNone ? R : lead > was || lead < was - kSpan ? lead + kRoom : was;
-                Info* const d = &s_info[it % kInfo];
-                uint32_t fl[4];
-                float kf[4], up[4], down[4];
+            const int was = R == kNone ? lead + kRoom : R;
+            const float move = R == kNone ? 1.0f : 0.0f;
+            R = lead == kNone ? R : lead > was || lead < was - kSpan ? lead + kRoom : was;
+            float kf[SUBS], up[SUBS], down[SUBS];
+            uint32_t flag[SUBS];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const int src = e / (4 / subs), lv = (int)(f4[src] >> 8 & 0xFF) - 127;
-                  fl[e] = (f4[src] & kThere) | (take >> src & 1 ? kTaken : 0u);
-                  kf[e] = pow2_byte(f4[src] & 0xFF);
-                  up[e] = (float)(8 + lv - R);
-                  down[e] = pow2i(R - lv - 8);
-                }
-                *reinterpret_cast<uint4*>(d->flags) = make_uint4(fl[0], fl[1], fl[2], fl[3]);
-                *reinterpret_cast<float4*>(d->kf) = make_float4(kf[0], kf[1], kf[2], kf[3]);
-                *reinterpret_cast<float4*>(d->up) = make_float4(up[0], up[1], up[2], up[3]);
-                *reinterpret_cast<float4*>(d->down) = make_float4(down[0], down[1], down[2], down[3]);
-                *reinterpret_cast<int4*>(&d->j0) = make_int4(j, i0 + i == tiles - 1 && !rem, R, __float_as_int(R == kNone ? 1.0f : pow2i(was - R)));
-                int there = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) there += p4[e] >= 0;
-                const int in_page = j & ((1 << t.page_shift) - 1);          // 0 but for pages of 128
-                mbar_expect_tx(kfull(s), (uint32_t)(there * rows_each * D));
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (p4[e] >= 0)
-                    tma_load_2d(k_at + s * C::kTileBytes + e * rows_each * D, &map_k, kfull(s), 0, ((p4[e] * t.n_kv_heads + head) << t.page_shift) + in_page);
-                ok = wait(vempty(v), ((it / kVStages) & 1) ^ 1);
-                if (ok) {
-                  mbar_expect_tx(vfull(v), (uint32_t)(there * rows_each * D));
-#pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    if (p4[e] >= 0)
-                      tma_load_2d(v_at + v * C::kTileBytes + e * rows_each * D, &map_v, vfull(v), 0, ((p4[e] * t.n_kv_heads + head) << t.page_shift) + in_page);
-                }
-              }
+            for (int e = 0; e < SUBS; ++e) {
+              const int lv = (int)(fl[e] >> 8 & 0xFF) - 127;
+              flag[e] = (fl[e] & kThere) | (take >> e & 1 ? kTaken : 0u);
+              kf[e] = pow2_byte(fl[e] & 0xFF);
+              up[e] = (float)(8 + lv - R);
+              down[e] = pow2i(R - lv - 8);
             }
-            ok = __shfl_sync(0xffffffffu, ok, 0);
+            constexpr int A2 = SUBS == 4 ? 1 : 0, C2 = SUBS / 2, D2 = SUBS - 1;   // the pages of keys 16 .. 31, 32 .. 47, 48 .. 63
+            const int s = it % kKStages, v = it % kVStages;
+            ok = __all_sync(0xffffffffu, wait(kempty(s), ((it / kKStages) & 1) ^ 1));
+            if (!ok) break;
+            if (elect_one()) {
+              Info* const d = &s_info[it % kInfo];
+              *reinterpret_cast<uint4*>(d->flags) = make_uint4(flag[0], flag[A2], flag[C2], flag[D2]);
+              *reinterpret_cast<float4*>(d->kf) = make_float4(kf[0], kf[A2], kf[C2], kf[D2]);
+              *reinterpret_cast<float4*>(d->up) = make_float4(up[0], up[A2], up[C2], up[D2]);
+              *reinterpret_cast<float4*>(d->down) = make_float4(down[0], down[A2], down[C2], down[D2]);
+              *reinterpret_cast<int4*>(&d->j0) = make_int4(j, i0 + i == tiles - 1 && !rem, R, __float_as_int(move != 0.0f ? move : pow2i(was - R)));
+              mbar_expect_tx(kfull(s), (uint32_t)(there * rows_each * D));
+#pragma unroll
+              for (int e = 0; e < SUBS; ++e)
+                if (line[e] >= 0) tma_load_2d(k_at + s * C::kTileBytes + e * rows_each * D, &map_k, kfull(s), 0, line[e]);
+            }
+            __syncwarp();
+            ok = __all_sync(0xffffffffu, wait(vempty(v), ((it / kVStages) & 1) ^ 1));
+            if (!ok) break;
+            if (elect_one()) {
+              mbar_expect_tx(vfull(v), (uint32_t)(there * rows_each * D));
+#pragma unroll
+              for (int e = 0; e < SUBS; ++e)
+                if (line[e] >= 0) tma_load_2d(v_at + v * C::kTileBytes + e * rows_each * D, &map_v, vfull(v), 0, line[e]);
+            }
+            __syncwarp();
             ++it;
           }
         }
@@ -633,7 +642,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   if (threadIdx.x == 0 && s_abort) report(t.status, B2Q_ERR_TIMEOUT);
 }
 
-template <int D>
+template <int D, int SUBS>
 int32_t launch(b2q_handle h, const AttendArgs& p) {
   using C = Cfg<D>;
   CUtensorMap map_k, map_v;
@@ -644,7 +653,7 @@ int32_t launch(b2q_handle h, const AttendArgs& p) {
   st = D == 128 ? b2q_tensor_map_2d(h, &map_v, p.v, 1, D, rows, D, box) : b2q_tensor_map_2d_sw64(h, &map_v, p.v, D, rows, box);
   if (st != B2Q_OK) return st;
   const int64_t units = (int64_t)p.t.tokens * p.group / kRows + p.t.seqs;
-  B2Q_SMEM_ATTR(h, kv8_prefill_kernel<D>, C::kSmem);
+  B2Q_SMEM_ATTR(h, (kv8_prefill_kernel<D, SUBS>), C::kSmem);
   // few row tiles against many keys: as many CTAs to a row tile as still find a place at once, each with eight key tiles at least
   const int64_t most = (int64_t)p.t.table_width << p.t.page_shift, keys = p.window ? p.window + kTile : most;
   int split = 1;
@@ -663,7 +672,7 @@ int32_t launch(b2q_handle h, const AttendArgs& p) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = h->sw.chain_pdl != 0 ? 2 : 1;
-  B2Q_CUDA(h, cudaLaunchKernelEx(&cfg, kv8_prefill_kernel<D>, map_k, map_v, p));
+  B2Q_CUDA(h, cudaLaunchKernelEx(&cfg, (kv8_prefill_kernel<D, SUBS>), map_k, map_v, p));
   return B2Q_OK;
 }
 
@@ -672,5 +681,7 @@ int32_t launch(b2q_handle h, const AttendArgs& p) {
 
 // The caller has checked the arguments; q_starts is not null.
 int32_t b2q_kv8_prefill(b2q_handle h, const kv8::AttendArgs& p, int64_t head_dim) {
-  return head_dim == 64 ? kv8::pre::launch<64>(h, p) : kv8::pre::launch<128>(h, p);
+  using namespace kv8::pre;
+  if (head_dim == 64) return p.t.page_shift >= 6 ? launch<64, 1>(h, p) : p.t.page_shift == 5 ? launch<64, 2>(h, p) : launch<64, 4>(h, p);
+  return p.t.page_shift >= 6 ? launch<128, 1>(h, p) : p.t.page_shift == 5 ? launch<128, 2>(h, p) : launch<128, 4>(h, p);
 }
