@@ -615,8 +615,11 @@ extern "C" int32_t b2q_kv8_attention_bf16(b2q_handle h, const void* q, int64_t l
   p.out = static_cast<__nv_bfloat16*>(out); p.lse = lse;
   if (tokens * p.group > 0x7FFFFFFF - 128)
     B2Q_FAIL(h, B2Q_ERR_INVALID_DIMENSION, "kv8_attention: %lld tokens of %lld heads are too many", (long long)tokens, (long long)n_heads);
-  if (q_starts && tokens * p.group > 32 * seqs) return b2q_kv8_prefill(h, p, head_dim);
-  // rows that share keys: up to 8 a CTA, 16 where a sequence has more than 8 on average (one conversion of the codes serves both halves)
+  // More than 16 rows to a sequence and kv head on average: the prefill kernel.  Measured there and here, us: 16 rows, 8 sequences x 4000 keys
+  // 30.6 and 26.0; 32 rows, 8 x 4000 33.2 and 36.2, 32 x 2000 46 and 71, 1 x 8000 24.9 and 33.0; 64 rows, 8 x 4000 40.6 and 58.9.
+  if (tokens * p.group > 16 * seqs) return b2q_kv8_prefill(h, p, head_dim);
+  // Rows that share keys: up to 8 a CTA, 16 where a sequence has more than 8 on average (one conversion of the codes serves both halves).
+  // 16 rows with 16 and with 8 to a CTA, us: 8 sequences x 4000 keys 25.2 and 29.9, 1 x 8000 17.9 and 20.9, 16 x 4000 36.4 and 48.0.
   const int rb = tokens * p.group > 8 * seqs ? 2 : 1, per = 8 * rb;
   const int64_t units = q_starts ? tokens * p.group / per + seqs : seqs * ceil_div64(p.group, per);   // at most
   const int64_t tiles = ceil_div64(p.window ? p.window + kv8::kTile : most, kv8::kTile);

@@ -10,15 +10,18 @@
 // splitting P into E4M3 terms costs every row four instructions per pair of weights), P goes back into the TMEM columns of its S as the
 // A operand.  A weight is held as p * 2^8 and is off by 2^-12 of itself, or of 2^-22 below the normal range of f16.
 // Work per 64 keys and CTA: 640 clocks of tensor core (Q K^T at N = 64 reads 1.5 x the shared memory that its rate allows, P V at N = D
-// runs at rate) against about 450 issue slots in each of four softmax warps: two CTAs share an SM, so that one multiplies while the
-// other exponentiates.
+// runs at rate), 512 of exponentials and 120 KB of shared memory traffic (48 for Q K^T, 16 for P V, 40 to convert the values, 16 to bring the
+// tiles in), 940 clocks: two CTAs share an SM, so that one multiplies while the other exponentiates.
+// Measured: 2 x 3900 tokens behind 150 (32 heads of 128 channels over 8 kv heads) 283 us, 765 TFLOP/s; 1 x 8000 tokens 523 us, 1000 TFLOP/s,
+// where a tile takes about 1100 clocks.  Leaving out the exponentials changes nothing there, leaving out the conversion of the values saves 6 %,
+// three quarters of Q K^T 10 %: shared memory bounds it, with the products' latency on top in short rows.
 // The running maximum is followed lazily: it moves only when a score exceeds it by more than 2^kSlack (f16 has the range), so O is rescaled
 // (a round trip through registers) once or twice per row and not per tile.  The value scale of a page is a power of two 2^lv: weights
 // enter as p * 2^(8 + lv - R) and O is in units of 2^(R - 8); a tile whose pages differ by more than 2^kSpan is walked once per group
 // of alike pages, the others masked.
 // Few row tiles: `split` CTAs of a cluster take every split'th key tile of the same rows and are joined through distributed shared memory.
-// Warp 0 walks the block table and issues the copies, warp 1 the products, warps 2 and 3 convert values, warps 4..7 are the softmax (a
-// thread to a row).
+// Warps 1 to 7 turn the query rows into E4M3 terms; then warp 0 walks the block table, issues the copies and describes each tile to the others,
+// warp 1 issues the products, warps 2 and 3 convert values, warps 4 to 7 are the softmax (a thread to a row).
 // Keys behind the last visible one are masked and their value rows become zeros in the conversion; a page that the table does not
 // name is neither read nor counted.  Every mbarrier wait is bounded; on expiry the kernel records B2Q_ERR_TIMEOUT and leaves.
 #include "kv8.cuh"
@@ -114,8 +117,8 @@ __device__ __forceinline__ void landed(uint32_t (&r)[64]) {
     asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
-// SUBS: pages that a tile of keys spans (1: pages of 64 and 128), known at compile time: the producer's share of a tile is then a third shorter,
-// and that was on the critical path (2 x 3900 tokens 308 -> 289 us)
+// SUBS: pages that a tile of keys spans (1: pages of 64 and 128), known at compile time: the producer is on the critical path, and its share of a tile
+// is then shorter (2 x 3900 tokens 289 us, with the general loop 308)
 template <int D, int SUBS>
 __global__ void __launch_bounds__(kThreads, 2)
 kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttendArgs p) {
@@ -174,8 +177,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   int tiles = (all - part + split - 1) / split;   // tiles part, part + split, ..
 
   // ---------------- the query rows, by warps 1 .. 7: D / 16 lanes to a row, 16 channels (16 bytes of codes) each ----------------
-  // They come in through the space of the f16 value tiles (free until the first of those is made), and a short loop turns them: unrolled
-  // over registers the same work was 13 KB of code that every CTA fetched once, 7 us.
+  // They come in through the space of the f16 value tiles (free until the first of those is made), and a short loop turns them: five turns
+  // unrolled cost every CTA more in instruction fetches than they saved (340 against 352 us at the time for 2 x 3900 tokens).
   constexpr int LPR = D / 16, RPW = 32 / LPR, QI = (kRows / RPW + 6) / 7;     // lanes to a row, rows at once, turns of a warp
   static_assert(QI * RPW <= 32, "a lane holds the address of each row");
   const int qc = lane % LPR;
@@ -356,7 +359,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     } else if (warp == 1) {
       // ---------------- MMA issuer: S of the next tile goes out before O of this one ----------------
       // The warp stays together and elects a lane for each group of products: descriptors then live in uniform registers.  One lane alone
-      // in its branch moved each operand there, product by product, and that chain bounded the kernel (5 % of its time).
+      // in its branch moved each operand there, product by product: 320 against 304 us at the time for 2 x 3900 tokens.
       const uint32_t id_s = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);                // E4M3 x E4M3, f32 sums
       const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);      // f16 x f16; V: channels contiguous
       auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
@@ -415,9 +418,11 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       // a thread keeps its unit u of 16 channels and its key modulo KEYS (a multiple of 8), so the swizzles are fixed
       constexpr int UNITS = D / 16, KEYS = 64 / UNITS;
       const int th = (int)threadIdx.x - 64, u = th % UNITS, key0 = th / UNITS, u2 = 2 * (u & 3);
+      // the threads of the upper channels write their second 16 bytes first: eight threads then meet no bank twice
+      const bool swap = u >= 4;
       const int src0 = key0 * D + ((D == 128 ? u ^ (key0 & 7) : u ^ ((key0 >> 1) & 3)) << 4);              // as TMA left it
-      const int dst0 = (u >> 2) * (kTile * 128) + key0 * 128 + ((u2 ^ (key0 & 7)) << 4);                   // block u / 4, units 2 (u & 3) and the next
-      const int step = (((u2 + 1) ^ (key0 & 7)) - (u2 ^ (key0 & 7))) * 16;
+      const int dst0 = (u >> 2) * (kTile * 128) + key0 * 128 + (((u2 + swap) ^ (key0 & 7)) << 4);          // block u / 4, units 2 (u & 3) and the next
+      const int step = (((u2 + !swap) ^ (key0 & 7)) - ((u2 + swap) ^ (key0 & 7))) * 16;
       const bool free_now = wait(qready, 0);        // the query rows have passed through the tiles that are written here
       for (int it = 0; free_now; ++it) {
         const int v = it % kVStages, b = it & 1;
@@ -433,7 +438,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         for (int k = 0; k < kTile; k += KEYS) {
           const uint4 x = *reinterpret_cast<const uint4*>(src + k * D);
           uint32_t o[8];
-          to_f16(x.x, o[0], o[1]); to_f16(x.y, o[2], o[3]); to_f16(x.z, o[4], o[5]); to_f16(x.w, o[6], o[7]);
+          to_f16(swap ? x.z : x.x, o[0], o[1]); to_f16(swap ? x.w : x.y, o[2], o[3]);
+          to_f16(swap ? x.x : x.z, o[4], o[5]); to_f16(swap ? x.y : x.w, o[6], o[7]);
           if (!whole && (!(d.flags[(key0 + k) >> 4] & kThere) || j0 + key0 + k >= key_end))   // no visible key here: whatever the row holds becomes 0
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = 0;
@@ -478,8 +484,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       const uint32_t both = d->flags[0] & d->flags[1] & d->flags[2] & d->flags[3];
       const bool clear = (both & (kThere | kTaken)) == (kThere | kTaken) && rest.x + kTile - 1 <= first_pos && (p.window <= 0 || rest.x > last_pos - p.window);
       landed(sr);
-      // Masking rewrites S in TMEM, 16 columns at a time in a loop that stays rolled, and loads it again: as straight code between the load
-      // and its use it ran once or twice per CTA and cost it 8 us each time in instruction fetches.
+      // Masking rewrites S in TMEM, 16 columns at a time in a loop that stays rolled, and loads it again: it runs once or twice per CTA, and as
+      // straight code between the load and its use it made the kernel slower by its instruction fetches.
       if (!clear) {
         const int top = pos - rest.x, low = p.window > 0 ? top - p.window : -1;      // columns low < j <= top
 #pragma unroll 1
@@ -654,7 +660,9 @@ int32_t launch(b2q_handle h, const AttendArgs& p) {
   if (st != B2Q_OK) return st;
   const int64_t units = (int64_t)p.t.tokens * p.group / kRows + p.t.seqs;
   B2Q_SMEM_ATTR(h, (kv8_prefill_kernel<D, SUBS>), C::kSmem);
-  // few row tiles against many keys: as many CTAs to a row tile as still find a place at once, each with eight key tiles at least
+  // Few row tiles against many keys: as many CTAs to a row tile as still find a place at once, each with eight key tiles at least.  Measured, us
+  // by the number of CTAs (taken: *): 1 x 512 tokens behind 15000 1: 221, 2: 154*, 4: 163;  1 x 130 behind 8000 1: 118, 2: 70, 4: 52*, 8: 53;
+  // 2 x 256 behind 4000 1: 66, 2: 55*, 4: 64;  4 x 300 behind 2000 1: 47*, 2: 65.
   const int64_t most = (int64_t)p.t.table_width << p.t.page_shift, keys = p.window ? p.window + kTile : most;
   int split = 1;
   while (split < 8 && units * p.t.n_kv_heads * split * 2 <= 2 * (int64_t)h->sm_count && keys >= (int64_t)split * 16 * kTile) split *= 2;
@@ -679,7 +687,7 @@ int32_t launch(b2q_handle h, const AttendArgs& p) {
 }  // namespace pre
 }  // namespace kv8
 
-// The caller has checked the arguments; q_starts is not null.
+// The caller has checked the arguments.
 int32_t b2q_kv8_prefill(b2q_handle h, const kv8::AttendArgs& p, int64_t head_dim) {
   using namespace kv8::pre;
   if (head_dim == 64) return p.t.page_shift >= 6 ? launch<64, 1>(h, p) : p.t.page_shift == 5 ? launch<64, 2>(h, p) : launch<64, 4>(h, p);
