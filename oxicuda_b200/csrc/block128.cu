@@ -7,9 +7,11 @@
 // float) and code = encode(v / scale).  Both are bound by HBM: every input is read once, every output written once.
 //
 // A block of 128 columns is 16 lanes of 8 elements (one 16-byte load each), so its absmax is four shuffles: no shared
-// memory, and the scale is known without a second pass.  Statistics and scales are f32; v / scale is v * (1 / scale) with
-// a correctly rounded reciprocal (one rounding more than a division, which shows only in codes that sit on a rounding
-// boundary; a division per element would make the kernels instruction-bound).
+// memory, and the scale is known without a second pass.  Statistics and scales are f32.  No element is divided (that would make the kernels
+// instruction-bound).  SwiGLU multiplies by the correctly rounded reciprocal of the scale.  The norm's quotient y / scale is
+// (r' gamma) * (max_val / absmax(r' gamma)): 1 / rms cancels, r' gamma is exact in f32 (two bf16), and the factor is held as a sum of two
+// floats, so that the quotient is rounded once; codes on the wrong side of a rounding boundary are then about six times fewer than where each
+// step of the formula is rounded.
 #include "common.cuh"
 
 namespace {
@@ -42,8 +44,7 @@ __device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ float block_scale(float amax, float max_val) {
   return amax > 0.0f ? fmaxf(__fdiv_rn(amax, max_val), kMinScale) : 1.0f;
 }
-__device__ __forceinline__ uint32_t encode1(float v, float inv_scale, int fmt, int rounding, const Fp8Fmt& F) {
-  float q = __fmul_rn(v, inv_scale);
+__device__ __forceinline__ uint32_t encode1(float q, int fmt, int rounding, const Fp8Fmt& F) {
   if (rounding == B2Q_ROUND_RNE) return fp8_encode_rne_dev(q, fmt);
   q = q < -F.max_val ? -F.max_val : (q > F.max_val ? F.max_val : q);
   return fp8_encode_ref_dev(q, F);
@@ -51,22 +52,22 @@ __device__ __forceinline__ uint32_t encode1(float v, float inv_scale, int fmt, i
 // What the kernels are compiled for: E4M3 to nearest even (the production form), or anything else (format and rounding at run time).
 enum Mode { kE4m3Rne, kAny };
 template <int MODE>
-__device__ __forceinline__ uint2 encode8(const uint64_t (&v)[4], float inv_scale, int fmt, int rounding, const Fp8Fmt& F) {
+__device__ __forceinline__ uint2 encode8(const uint64_t (&q)[4], int fmt, int rounding, const Fp8Fmt& F) {
   if (MODE == kE4m3Rne) {                      // the conversion saturates to +-448 by itself
-    const uint64_t inv = pair(inv_scale, inv_scale);
     uint32_t p[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint64_t q = mul2(v[j], inv);
-      p[j] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo(q), hi(q)), __NV_SATFINITE, __NV_E4M3);
-    }
+    for (int j = 0; j < 4; ++j) p[j] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo(q[j]), hi(q[j])), __NV_SATFINITE, __NV_E4M3);
     return make_uint2(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410));
   }
   uint32_t w[2] = {0, 0};
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    w[j >> 1] |= (encode1(lo(v[j]), inv_scale, fmt, rounding, F) | encode1(hi(v[j]), inv_scale, fmt, rounding, F) << 8) << (16 * (j & 1));
+  for (int j = 0; j < 4; ++j) w[j >> 1] |= (encode1(lo(q[j]), fmt, rounding, F) | encode1(hi(q[j]), fmt, rounding, F) << 8) << (16 * (j & 1));
   return make_uint2(w[0], w[1]);
+}
+template <int MODE>
+__device__ __forceinline__ uint2 encode8(const uint64_t (&v)[4], float inv_scale, int fmt, int rounding, const Fp8Fmt& F) {
+  const uint64_t inv = pair(inv_scale, inv_scale), q[4] = {mul2(v[0], inv), mul2(v[1], inv), mul2(v[2], inv), mul2(v[3], inv)};
+  return encode8<MODE>(q, fmt, rounding, F);
 }
 // max over the 16 lanes that hold one block of 128 columns
 __device__ __forceinline__ float max16(float v) {
@@ -92,6 +93,22 @@ __device__ __forceinline__ void block_scales(const float (&amax)[N], float max_v
   const float r = __frcp_rn(mine);
 #pragma unroll
   for (int k = 0; k < N; ++k) inv[k] = N == 1 ? r : __shfl_sync(0xffffffffu, r, (lane & 16) | k);
+}
+// The norm's scale of a block whose largest |r' gamma| is amax, and the factor hi + lo that takes r' gamma to codes; hi = 0: the block is outside
+// the range in which no step over- or underflows, and is done by the formula's own steps.
+struct NormScale { float scale, hi, lo; };
+__device__ __forceinline__ NormScale norm_scale(float amax, float inv_rms, float max_val) {
+  NormScale n{block_scale(__fmul_rn(amax, inv_rms), max_val), 0.0f, 0.0f};
+  if (inv_rms >= 0x1p-60f && inv_rms <= 0x1p60f) {
+    if (amax == 0.0f) n.hi = 1.0f;
+    else if (amax >= 0x1p-60f && amax <= 0x1p100f && n.scale > kMinScale) {
+      float inv;                                           // any quotient will do: the remainder is exact
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(amax));
+      n.hi = __fmul_rn(max_val, inv);
+      n.lo = __fmul_rn(fmaf(-n.hi, amax, max_val), inv);
+    }
+  }
+  return n;
 }
 __device__ __forceinline__ float block_sum(float v, float* sh) {
 #pragma unroll
@@ -155,8 +172,8 @@ __global__ void __launch_bounds__(1024) rms_norm_block128_kernel(const NormArgs 
   const Fp8Fmt F = fp8_fmt(p.fmt);
   uint2* cr = reinterpret_cast<uint2*>(p.codes + r * p.cols);
   uint4* yr = p.y ? reinterpret_cast<uint4*>(p.y + r * p.cols) : nullptr;
-  uint64_t v[NCH][4];
-  float amax[NCH], inv[NCH], mine;
+  uint64_t v[NCH][4];                                      // r' gamma
+  float amax[NCH];
 #pragma unroll
   for (int k = 0; k < NCH; ++k) {
     const int c = (int)threadIdx.x + k * (int)blockDim.x;
@@ -164,20 +181,54 @@ __global__ void __launch_bounds__(1024) rms_norm_block128_kernel(const NormArgs 
     unpack8(c < chunks ? __ldg(gr + c) : make_uint4(0, 0, 0, 0), g);
     unpack8(xq[k], v[k]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[k][j] = mul2(mul2(v[k][j], inv2), g[j]);
-    amax[k] = max16(c < chunks ? absmax8(v[k]) : 0.0f);    // (0 * inf behind the row's end would be a NaN, which the maximum passes over)
+    for (int j = 0; j < 4; ++j) v[k][j] = mul2(v[k][j], g[j]);
+    amax[k] = max16(absmax8(v[k]));
   }
-  block_scales<NCH>(amax, F.max_val, mine, inv);
+  // lane k of a group of 16 makes the scale of the group's k'th block
+  const int lane = threadIdx.x & 31, sub = lane & 15;
+  float a = amax[0];
+#pragma unroll
+  for (int k = 1; k < NCH; ++k) a = sub == k ? amax[k] : a;
+  const NormScale mine = norm_scale(a, inv_rms, F.max_val);
 #pragma unroll
   for (int k = 0; k < NCH; ++k) {
     const int c = (int)threadIdx.x + k * (int)blockDim.x;
-    if ((threadIdx.x & 15) == k && (c & ~15) < chunks) p.scales[r * nb + (c >> 4)] = mine;
-    if (c < chunks) {
-      cr[c] = encode8<MODE>(v[k], inv[k], p.fmt, p.rounding, F);
-      if (yr)
-        yr[c] = make_uint4(bf16_pair(lo(v[k][0]), hi(v[k][0])), bf16_pair(lo(v[k][1]), hi(v[k][1])), bf16_pair(lo(v[k][2]), hi(v[k][2])),
-                           bf16_pair(lo(v[k][3]), hi(v[k][3])));
+    const float fh = NCH == 1 ? mine.hi : __shfl_sync(0xffffffffu, mine.hi, (lane & 16) | k), fl = NCH == 1 ? mine.lo : __shfl_sync(0xffffffffu, mine.lo, (lane & 16) | k);
+    float scale = mine.scale;                              // of lane k alone
+    if (fh != 0.0f) {
+      if (yr && c < chunks) {                              // by the formula's steps: r' gamma of an element far below its block's largest may be subnormal
+        uint64_t g[4], y[4];
+        unpack8(__ldg(gr + c), g);
+        unpack8(rr ? rr[c] : xr[c], y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = mul2(mul2(y[j], inv2), g[j]);
+        yr[c] = make_uint4(bf16_pair(lo(y[0]), hi(y[0])), bf16_pair(lo(y[1]), hi(y[1])), bf16_pair(lo(y[2]), hi(y[2])), bf16_pair(lo(y[3]), hi(y[3])));
+      }
+      const uint64_t h2 = pair(fh, fh), l2 = pair(fl, fl);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint64_t q = mul2(v[k][j], l2);
+        fma2(q, v[k][j], h2);
+        v[k][j] = q;
+      }
+      if (c < chunks) cr[c] = encode8<MODE>(v[k], p.fmt, p.rounding, F);
+    } else {                                               // all 16 lanes of the block
+      uint64_t g[4], y[4];
+      unpack8(c < chunks ? gr[c] : make_uint4(0, 0, 0, 0), g);
+      unpack8(c < chunks ? (rr ? rr[c] : xr[c]) : make_uint4(0, 0, 0, 0), y);
+      float top = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = mul2(mul2(y[j], inv2), g[j]);
+      if (c < chunks) top = absmax8(y);                    // (0 * inf behind the row's end would be a NaN, which the maximum passes over)
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFu << (lane & 16), top, o));
+      scale = block_scale(top, F.max_val);
+      if (c < chunks) {
+        cr[c] = encode8<MODE>(y, __frcp_rn(scale), p.fmt, p.rounding, F);
+        if (yr) yr[c] = make_uint4(bf16_pair(lo(y[0]), hi(y[0])), bf16_pair(lo(y[1]), hi(y[1])), bf16_pair(lo(y[2]), hi(y[2])), bf16_pair(lo(y[3]), hi(y[3])));
+      }
     }
+    if (sub == k && (c & ~15) < chunks) p.scales[r * nb + (c >> 4)] = scale;
   }
 }
 
@@ -205,21 +256,42 @@ __global__ void __launch_bounds__(256) rms_norm_block128_generic_kernel(const No
   const int64_t nb = (p.cols + 127) >> 7;
   const int lane = threadIdx.x & 31;
   for (int64_t b = threadIdx.x >> 5; b < nb; b += blockDim.x >> 5) {
-    float v[4], amax = 0.0f;
+    float w[4], g[4], amax = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t i = b * 128 + j * 32 + lane;
-      v[j] = i < p.cols ? __fmul_rn(__fmul_rn(__bfloat162float(src[i]), inv_rms), __bfloat162float(p.gamma[i])) : 0.0f;
-      amax = fmaxf(amax, fabsf(v[j]));
+      w[j] = i < p.cols ? __bfloat162float(src[i]) : 0.0f;
+      g[j] = i < p.cols ? __bfloat162float(p.gamma[i]) : 0.0f;
+      amax = fmaxf(amax, fabsf(__fmul_rn(w[j], g[j])));
     }
-    const float scale = block_scale(warp_max(amax), F.max_val), inv = __frcp_rn(scale);
+    const NormScale n = norm_scale(warp_max(amax), inv_rms, F.max_val);
+    float scale = n.scale, q[4], y[4];
+    if (n.hi != 0.0f) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float v = __fmul_rn(w[j], g[j]);
+        y[j] = __fmul_rn(__fmul_rn(w[j], inv_rms), g[j]);
+        q[j] = fmaf(v, n.hi, __fmul_rn(v, n.lo));
+      }
+    } else {
+      amax = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        y[j] = __fmul_rn(__fmul_rn(w[j], inv_rms), g[j]);
+        if (b * 128 + j * 32 + lane < p.cols) amax = fmaxf(amax, fabsf(y[j]));
+      }
+      scale = block_scale(warp_max(amax), F.max_val);
+      const float inv = __frcp_rn(scale);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[j] = __fmul_rn(y[j], inv);
+    }
     if (lane == 0) p.scales[r * nb + b] = scale;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t i = b * 128 + j * 32 + lane;
       if (i < p.cols) {
-        p.codes[r * p.cols + i] = (uint8_t)encode1(v[j], inv, p.fmt, p.rounding, F);
-        if (p.y) p.y[r * p.cols + i] = __float2bfloat16_rn(v[j]);
+        p.codes[r * p.cols + i] = (uint8_t)encode1(q[j], p.fmt, p.rounding, F);
+        if (p.y) p.y[r * p.cols + i] = __float2bfloat16_rn(y[j]);
       }
     }
   }
@@ -327,7 +399,7 @@ __global__ void __launch_bounds__(256) swiglu_block128_generic_kernel(const Swig
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t c = b * 128 + j * 32 + lane;
-      if (c < p.cols) p.codes[r * p.cols + c] = (uint8_t)encode1(h[j], inv, p.fmt, p.rounding, F);
+      if (c < p.cols) p.codes[r * p.cols + c] = (uint8_t)encode1(__fmul_rn(h[j], inv), p.fmt, p.rounding, F);
     }
   }
 }

@@ -130,6 +130,7 @@ gemm_block128_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer: one accumulator per block of K; the warp stays together and elects a lane (descriptors in uniform registers) ----------------
+    asm volatile("griddepcontrol.wait;" ::: "memory");                  // the limit of a wait counts from the end of the previous kernel
     bool ok = true;
     for (int it = 0; it < total; ++it) {
       const int s = it % kStages, b = it % kBuf;
@@ -185,6 +186,7 @@ gemm_block128_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
     }
   } else {
     // ---------------- epilogue: this thread's weight row is TMEM lane 32 (warp & 3) + lane ----------------
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     for (int it = 0, i = 0; it < total; ++it) {
       const int b = it % kBuf, slot = i % C::kSlots;

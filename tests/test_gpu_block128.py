@@ -86,6 +86,40 @@ def test_norm_and_swiglu_formats(cuda, fmt, rounding):
             _check_codes(h, *swiglu_quantize_fp8_block128(x, up, fmt=fmt), fmt)
 
 
+@pytest.mark.parametrize("cols", [1024, 8192, 16384, 1031])
+def test_norm_far_from_one(cuda, cols):
+    """Rows and weights whose product leaves the range of f32, or comes near its ends, beside ordinary ones."""
+    from oxicuda_b200.kv_cache import rms_norm_quantize_fp8_block128
+    g = torch.Generator(device=cuda).manual_seed(cols)
+    size = torch.tensor([1.0, 2.0 ** -60, 2.0 ** 50, 2.0 ** -30, 2.0 ** 30, 1.0], device=cuda)
+    x = (torch.randn(6, cols, device=cuda, generator=g) * size[:, None]).to(torch.bfloat16)
+    gain = torch.exp2(torch.tensor([0.0, -90.0, 100.0, -60.0, 40.0, -20.0, 20.0, 0.0], device=cuda)).repeat_interleave(-(-cols // 8))[:cols]
+    gamma = (torch.randn(cols, device=cuda, generator=g).clamp(min=0.05) * gain).to(torch.bfloat16)
+    for eps in (0.0, 1e-5):
+        codes, scales, yy = rms_norm_quantize_fp8_block128(x, gamma, eps, want_y=True)
+        v = x.double()
+        y = v / torch.sqrt((v * v).mean(dim=1, keepdim=True) + eps) * gamma.double()
+        _check_codes(y, codes, scales)
+        assert ((yy.double() - y).abs() <= (2.0 ** -8 + 1e-5) * y.abs() + 2.0 ** -126).all()
+
+
+def test_norm_codes_are_those_of_the_exact_quotients(cuda):
+    """The quotient is rounded once before it is encoded: a code differs from the exact quotient's only where that lies within 2^-23 of itself
+    from the middle between two codes."""
+    from oxicuda_b200.kv_cache import rms_norm_quantize_fp8_block128
+    g = torch.Generator(device=cuda).manual_seed(77)
+    x, gamma = torch.randn(200, 4096, device=cuda, generator=g).to(torch.bfloat16), (1 + 0.1 * torch.randn(4096, device=cuda, generator=g)).to(torch.bfloat16)
+    codes, _ = rms_norm_quantize_fp8_block128(x, gamma, 1e-5)
+    w = (x.double() * gamma.double()).view(200, 32, 128)
+    q = (w * (448.0 / w.abs().amax(dim=2, keepdim=True))).view(200, 4096)
+    grid = torch.arange(127, dtype=torch.uint8, device=cuda).view(torch.float8_e4m3fn).double()
+    hi = torch.searchsorted(grid, q.abs()).clamp(1, 126)
+    mid = (grid[hi] + grid[hi - 1]) / 2
+    clear = (q.abs() - mid).abs() > 2.0 ** -23 * q.abs()
+    want = torch.where(q.abs() > mid, grid[hi], grid[hi - 1]) * torch.sign(q)
+    assert torch.equal(_values(codes)[clear], want[clear]) and clear.double().mean() > 0.999
+
+
 def test_norm_of_non_finite_rows(cuda):
     """A row with a NaN is NaN throughout, a row with an infinity zeros and NaN (x / inf); the rows beside them are untouched."""
     from oxicuda_b200.kv_cache import rms_norm_quantize_fp8_block128
