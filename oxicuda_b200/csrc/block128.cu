@@ -8,10 +8,11 @@
 //
 // A block of 128 columns is 16 lanes of 8 elements (one 16-byte load each), so its absmax is four shuffles: no shared
 // memory, and the scale is known without a second pass.  Statistics and scales are f32.  No element is divided (that would make the kernels
-// instruction-bound).  SwiGLU multiplies by the correctly rounded reciprocal of the scale.  The norm's quotient y / scale is
-// (r' gamma) * (max_val / absmax(r' gamma)): 1 / rms cancels, r' gamma is exact in f32 (two bf16), and the factor is held as a sum of two
-// floats, so that the quotient is rounded once; codes on the wrong side of a rounding boundary are then about six times fewer than where each
-// step of the formula is rounded.
+// instruction-bound): v / scale is v * (max_val / absmax), the factor held as a sum of two floats, so that the quotient is rounded once.  In the
+// norm it is (r' gamma) * (max_val / absmax(r' gamma)): 1 / rms cancels and r' gamma is exact in f32 (two bf16).  Of 7.4 million codes of a
+// norm none then differs from the exact quotient's; with each step of the formula rounded 641 did.  In SwiGLU the hardware's exponential is
+// what is left: 2 codes in a million, as with the formula in f32 (a Newton step for the reciprocal and an exponent in two parts changed
+// neither that nor anything else but the time, 50 to 60 us for 2047 x 28672).
 #include "common.cuh"
 
 namespace {
@@ -64,6 +65,15 @@ __device__ __forceinline__ uint2 encode8(const uint64_t (&q)[4], int fmt, int ro
   for (int j = 0; j < 4; ++j) w[j >> 1] |= (encode1(lo(q[j]), fmt, rounding, F) | encode1(hi(q[j]), fmt, rounding, F) << 8) << (16 * (j & 1));
   return make_uint2(w[0], w[1]);
 }
+// v (hi + lo), rounded once
+__device__ __forceinline__ void scale8(const uint64_t (&v)[4], float hi, float lo, uint64_t (&q)[4]) {
+  const uint64_t h2 = pair(hi, hi), l2 = pair(lo, lo);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    q[j] = mul2(v[j], l2);
+    fma2(q[j], v[j], h2);
+  }
+}
 template <int MODE>
 __device__ __forceinline__ uint2 encode8(const uint64_t (&v)[4], float inv_scale, int fmt, int rounding, const Fp8Fmt& F) {
   const uint64_t inv = pair(inv_scale, inv_scale), q[4] = {mul2(v[0], inv), mul2(v[1], inv), mul2(v[2], inv), mul2(v[3], inv)};
@@ -81,34 +91,40 @@ __device__ __forceinline__ float absmax8(const uint64_t (&v)[4]) {
   for (int j = 0; j < 4; ++j) a = fmaxf(a, fmaxf(fabsf(lo(v[j])), fabsf(hi(v[j]))));
   return a;
 }
-// The scales of the N blocks that a group of 16 lanes holds: lane k of the group makes the k'th (a division and a reciprocal are some
-// twenty instructions each), the others get its reciprocal.  `mine` is the scale that this lane made (k < N).
-template <int N>
-__device__ __forceinline__ void block_scales(const float (&amax)[N], float max_val, float& mine, float (&inv)[N]) {
-  const int lane = threadIdx.x & 31, sub = lane & 15;
-  float a = amax[0];
-#pragma unroll
-  for (int k = 1; k < N; ++k) a = sub == k ? amax[k] : a;
-  mine = block_scale(a, max_val);
-  const float r = __frcp_rn(mine);
-#pragma unroll
-  for (int k = 0; k < N; ++k) inv[k] = N == 1 ? r : __shfl_sync(0xffffffffu, r, (lane & 16) | k);
-}
 // The norm's scale of a block whose largest |r' gamma| is amax, and the factor hi + lo that takes r' gamma to codes; hi = 0: the block is outside
 // the range in which no step over- or underflows, and is done by the formula's own steps.
 struct NormScale { float scale, hi, lo; };
+// max_val / amax as a sum of two floats (amax from 2^-100 to 2^100)
+__device__ __forceinline__ void quotient(float max_val, float amax, float& hi, float& lo) {
+  float inv;                                               // any quotient will do: the remainder is exact
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(amax));
+  hi = __fmul_rn(max_val, inv);
+  lo = __fmul_rn(fmaf(-hi, amax, max_val), inv);
+}
 __device__ __forceinline__ NormScale norm_scale(float amax, float inv_rms, float max_val) {
   NormScale n{block_scale(__fmul_rn(amax, inv_rms), max_val), 0.0f, 0.0f};
   if (inv_rms >= 0x1p-60f && inv_rms <= 0x1p60f) {
     if (amax == 0.0f) n.hi = 1.0f;
-    else if (amax >= 0x1p-60f && amax <= 0x1p100f && n.scale > kMinScale) {
-      float inv;                                           // any quotient will do: the remainder is exact
-      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(amax));
-      n.hi = __fmul_rn(max_val, inv);
-      n.lo = __fmul_rn(fmaf(-n.hi, amax, max_val), inv);
-    }
+    else if (amax >= 0x1p-60f && amax <= 0x1p100f && n.scale > kMinScale) quotient(max_val, amax, n.hi, n.lo);
   }
   return n;
+}
+// The scales of the N blocks that a group of 16 lanes holds: lane k of the group makes the k'th (a division is some ten instructions), the
+// others get the factor hi + lo that takes its elements to codes.  `mine` is the scale that this lane made (k < N).
+template <int N>
+__device__ __forceinline__ void block_scales(const float (&amax)[N], float max_val, float& mine, float (&fh)[N], float (&fl)[N]) {
+  const int lane = threadIdx.x & 31, sub = lane & 15;
+  float a = amax[0], h, l = 0.0f;
+#pragma unroll
+  for (int k = 1; k < N; ++k) a = sub == k ? amax[k] : a;
+  mine = block_scale(a, max_val);
+  if (a >= 0x1p-100f && a <= 0x1p100f) quotient(max_val, a, h, l);
+  else h = __frcp_rn(mine);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    fh[k] = __shfl_sync(0xffffffffu, h, (lane & 16) | k);
+    fl[k] = __shfl_sync(0xffffffffu, l, (lane & 16) | k);
+  }
 }
 __device__ __forceinline__ float block_sum(float v, float* sh) {
 #pragma unroll
@@ -204,14 +220,9 @@ __global__ void __launch_bounds__(1024) rms_norm_block128_kernel(const NormArgs 
         for (int j = 0; j < 4; ++j) y[j] = mul2(mul2(y[j], inv2), g[j]);
         yr[c] = make_uint4(bf16_pair(lo(y[0]), hi(y[0])), bf16_pair(lo(y[1]), hi(y[1])), bf16_pair(lo(y[2]), hi(y[2])), bf16_pair(lo(y[3]), hi(y[3])));
       }
-      const uint64_t h2 = pair(fh, fh), l2 = pair(fl, fl);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint64_t q = mul2(v[k][j], l2);
-        fma2(q, v[k][j], h2);
-        v[k][j] = q;
-      }
-      if (c < chunks) cr[c] = encode8<MODE>(v[k], p.fmt, p.rounding, F);
+      uint64_t q[4];
+      scale8(v[k], fh, fl, q);
+      if (c < chunks) cr[c] = encode8<MODE>(q, p.fmt, p.rounding, F);
     } else {                                               // all 16 lanes of the block
       uint64_t g[4], y[4];
       unpack8(c < chunks ? gr[c] : make_uint4(0, 0, 0, 0), g);
@@ -351,7 +362,7 @@ __global__ void __launch_bounds__(256) swiglu_block128_kernel(const SwigluArgs p
       }
     }
     uint64_t h[2][4];
-    float amax[2], inv[2], mine;
+    float amax[2], fh[2], fl[2], mine;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       uint64_t g[4], u[4];
@@ -370,11 +381,13 @@ __global__ void __launch_bounds__(256) swiglu_block128_kernel(const SwigluArgs p
         amax[k] = max16(absmax8(h[k]));
       }
     }
-    block_scales<2>(amax, F.max_val, mine, inv);
+    block_scales<2>(amax, F.max_val, mine, fh, fl);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       if (sub == k && at[k] < total) p.scales[at[k]] = mine;
-      if (live[k]) *reinterpret_cast<uint2*>(p.codes + row[k] * p.cols + col[k]) = encode8<MODE>(h[k], inv[k], p.fmt, p.rounding, F);
+      uint64_t q[4];
+      scale8(h[k], fh[k], fl[k], q);
+      if (live[k]) *reinterpret_cast<uint2*>(p.codes + row[k] * p.cols + col[k]) = encode8<MODE>(q, p.fmt, p.rounding, F);
     }
   }
 }

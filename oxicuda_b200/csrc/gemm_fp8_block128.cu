@@ -8,6 +8,8 @@
 // flight), and eight epilogue warps per CTA add scale * product to sums that they hold in registers (BN / 2 columns of one row
 // per thread) while the tensor core works on the next blocks.  Per block and CTA the tensor core needs 128 x BN x 128 / 8192 =
 // 2 BN clocks; the epilogue reads BN columns of TMEM and issues BN / 2 two-wide FMAs per warp scheduler, which fits beside it.
+// Measured: 4096 x 8192 x 28672 831 to 853 us (2.3 PFLOP/s, two thirds of the FP8 rate; the power cap acts), 2048 x 8192 x 8192 127 us (2.2),
+// 512 x 8192 x 8192 35 us (1.9).
 #include "tc_common.cuh"
 
 namespace b128 {
@@ -87,6 +89,10 @@ struct Params {
 using namespace tcx;
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   return mbar_wait_bounded(bar, parity, abort_flag, kWaitLimitNs, 1);
+}
+// By a whole warp, whose lanes leave together if one gives up.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 __device__ __forceinline__ void umma_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -193,7 +199,7 @@ gemm_block128_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
         for (int u = pair; u < total && ok; u += num_pairs) {
           for (int kb = 0; kb < num_kb; ++kb, ++it) {
             const int s = it % kStages, b = it % kBuf;
-            ok = __all_sync(0xffffffffu, mbar_wait(tempty_bar(b), ((it / kBuf) & 1) ^ 1, abort_flag) && mbar_wait(full_bar(s), (it / kStages) & 1, abort_flag));
+            ok = warp_wait(tempty_bar(b), ((it / kBuf) & 1) ^ 1, abort_flag) && warp_wait(full_bar(s), (it / kStages) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
@@ -236,7 +242,7 @@ gemm_block128_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
           float4 w4[C::kColBlocks];
 #pragma unroll
           for (int c = 0; c < C::kColBlocks; ++c) w4[c] = load4(sw[c], k0, num_kb, p.vec);
-          if (!mbar_wait(sempty_bar(s), ((it / C::kSlots) & 1) ^ 1, abort_flag)) { ok = false; break; }
+          if (!warp_wait(sempty_bar(s), ((it / C::kSlots) & 1) ^ 1, abort_flag)) { ok = false; break; }
           float* d = s_scale + s * (C::kSlotBytes / 4) + r0;
 #pragma unroll
           for (int c = 0; c < C::kColBlocks; ++c) {
@@ -263,7 +269,7 @@ gemm_block128_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
     for (int u = pair; u < total && ok; u += num_pairs) {
       int mb, nb;
       tile_coords(u, p, mb, nb);
-      const int64_t m_warp0 = (int64_t)mb * 256 + rank * BM + q * 32, m = m_warp0 + lane;
+      const int64_t m_warp0 = (int64_t)mb * 256 + rank * BM + q * 32;
       const int64_t n0 = (int64_t)nb * BN + half * HALF;
       uint64_t acc[NACC];
 #pragma unroll
@@ -271,8 +277,8 @@ gemm_block128_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
       const float* my_scale = s_scale + (BN == 256 ? half * BM : 0) + q * 32 + lane;
       for (int kb = 0; kb < num_kb; ++kb, ++it) {
         const int b = it % kBuf, slot = sit % C::kSlots;
-        if ((kb & 3) == 0 && !mbar_wait(sfull_bar(slot), (sit / C::kSlots) & 1, abort_flag)) { ok = false; break; }
-        if (!mbar_wait(tfull_bar(b), (it / kBuf) & 1, abort_flag)) { ok = false; break; }
+        if ((kb & 3) == 0 && !warp_wait(sfull_bar(slot), (sit / C::kSlots) & 1, abort_flag)) { ok = false; break; }
+        if (!warp_wait(tfull_bar(b), (it / kBuf) & 1, abort_flag)) { ok = false; break; }
         __syncwarp();
         tc_fence_after();
         const uint32_t t = tmem_base + b * BN + half * HALF + ((uint32_t)(q * 32) << 16);
@@ -336,13 +342,29 @@ gemm_block128_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
             if (lane == 0 && n0 + x < p.N) { tma_store_2d(&map_out, stage, (int)(n0 + x), (int)m_warp0); tma_store_commit(); }
           }
         }
-      } else if (m < p.M) {                                            // pitches that TMA cannot take: stores from registers
+      } else {
+        // Pitches that TMA cannot take: 32 x 32 results through the same buffer, then row by row, a column to a lane.  (2973 x 13158 x 608 in f32
+        // takes 58 us; with a row to a lane, its stores scattered over 32 rows, it took 300.)
+        uint8_t* const row = stage_p + lane * 128;
+        const int rows = (int)(p.M - m_warp0 < 32 ? p.M - m_warp0 : 32);
 #pragma unroll
-        for (int j = 0; j < HALF; ++j) {
-          const float v = (j & 1) ? hi32(acc[j / 2]) : lo32(acc[j / 2]);
-          if (n0 + j < p.N) {
-            if (p.out_type == B2Q_OUT_BF16) reinterpret_cast<__nv_bfloat16*>(p.out)[m * p.N + n0 + j] = __float2bfloat16_rn(v);
-            else reinterpret_cast<float*>(p.out)[m * p.N + n0 + j] = v;
+        for (int x = 0; x < HALF; x += 32) {
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const uint64_t v0 = acc[(x + j) / 2], v1 = acc[(x + j) / 2 + 1];
+            *reinterpret_cast<float4*>(row + (((j >> 2) ^ (lane & 7)) << 4)) = make_float4(lo32(v0), hi32(v0), lo32(v1), hi32(v1));
+          }
+          __syncwarp();
+          const int64_t n = n0 + x + lane;
+          if (n < p.N) {
+#pragma unroll 4
+            for (int i = 0; i < rows; ++i) {
+              const float v = *reinterpret_cast<const float*>(stage_p + i * 128 + (((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4);
+              const int64_t at = (m_warp0 + i) * p.N + n;
+              if (p.out_type == B2Q_OUT_BF16) reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+              else reinterpret_cast<float*>(p.out)[at] = v;
+            }
           }
         }
       }

@@ -288,8 +288,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const int mk = key_of<D>(lr), ve[2] = {key_of<D>(2 * tq), key_of<D>(2 * tq + 1)};   // this lane's key row, its two value rows (mod 8)
     for (int it = warp >> 1; it < mine; it += kWarps / 2) {
       const int st = it % G::kStages, j0 = key_begin + kTile * (part + split * it) + 32 * (warp & 1);   // this warp's 32 keys
-      if (!mbar_wait_bounded(full_bar(st), (it / G::kStages) & 1, abort_flag, kWaitLimitNs, 1)) break;
-      __syncwarp();
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(full_bar(st), (it / G::kStages) & 1, abort_flag, kWaitLimitNs, 1))) break;
       const uint8_t* const ks = ring + st * G::kStage + 32 * (warp & 1) * D;
       uint8_t* const vs = ring + st * G::kStage + G::kHalf + 32 * (warp & 1) * D;
       const uint2 info = reinterpret_cast<const uint2*>(s_info + st)[warp & 1];

@@ -208,7 +208,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem_base, 0), tmem_o = tmem + 2 * kTile;
   volatile int* abort_flag = &s_abort;
-  auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, abort_flag, kWaitLimitNs, 1); };
+  // by whole warps, which leave together if one lane gives up
+  auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, kWaitLimitNs, 1)); };
 
   if (warp > 0) {
     const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
@@ -324,7 +325,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             }
             constexpr int A2 = SUBS == 4 ? 1 : 0, C2 = SUBS / 2, D2 = SUBS - 1;   // the pages of keys 16 .. 31, 32 .. 47, 48 .. 63
             const int s = it % kKStages, v = it % kVStages;
-            ok = __all_sync(0xffffffffu, wait(kempty(s), ((it / kKStages) & 1) ^ 1));
+            ok = wait(kempty(s), ((it / kKStages) & 1) ^ 1);
             if (!ok) break;
             if (elect_one()) {
               Info* const d = &s_info[it % kInfo];
@@ -339,7 +340,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
                 if (line[e] >= 0) tma_load_2d(k_at + s * C::kTileBytes + e * rows_each * D, &map_k, kfull(s), 0, line[e]);
             }
             __syncwarp();
-            ok = __all_sync(0xffffffffu, wait(vempty(v), ((it / kVStages) & 1) ^ 1));
+            ok = wait(vempty(v), ((it / kVStages) & 1) ^ 1);
             if (!ok) break;
             if (elect_one()) {
               mbar_expect_tx(vfull(v), (uint32_t)(there * rows_each * D));
@@ -362,11 +363,10 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       // in its branch moved each operand there, product by product: 320 against 304 us at the time for 2 x 3900 tokens.
       const uint32_t id_s = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);                // E4M3 x E4M3, f32 sums
       const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);      // f16 x f16; V: channels contiguous
-      auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
-      bool ok = all_wait(qready, 0);
+      bool ok = wait(qready, 0);
       auto scores = [&](int it) {
         const int s = it % kKStages, b = it & 1;
-        if (!all_wait(kfull(s), (it / kKStages) & 1)) return false;
+        if (!wait(kfull(s), (it / kKStages) & 1)) return false;
         tc_fence_after();
         if (elect_one()) {
           const uint32_t kt = k_at + s * C::kTileBytes;
@@ -387,9 +387,9 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       for (int it = 0; ok; ++it) {
         const int last = __shfl_sync(0xffffffffu, s_info[it % kInfo].last, 0);   // written before the tile's copies were issued, which scores(it) waited for
         // S of tile it + 1 overwrites S and P of tile it - 1: their product has to be done
-        if (!last && !(ok = (it == 0 || all_wait(pvdone, (it - 1) & 1)) && scores(it + 1))) break;
+        if (!last && !(ok = (it == 0 || wait(pvdone, (it - 1) & 1)) && scores(it + 1))) break;
         const int b = it & 1;
-        if (!all_wait(wfull(b), (it >> 1) & 1) || !all_wait(pfull(b), (it >> 1) & 1)) { ok = false; break; }
+        if (!wait(wfull(b), (it >> 1) & 1) || !wait(pfull(b), (it >> 1) & 1)) { ok = false; break; }
         tc_fence_after();
         if (elect_one()) {
           const uint32_t vt = w_at + b * C::kV16;
@@ -427,7 +427,6 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       for (int it = 0; free_now; ++it) {
         const int v = it % kVStages, b = it & 1;
         if (!wait(vfull(v), (it / kVStages) & 1) || !wait(wempty(b), ((it >> 1) & 1) ^ 1)) break;
-        __syncwarp();
         const Info& d = s_info[it % kInfo];
         const uint32_t flags[4] = {d.flags[0], d.flags[1], d.flags[2], d.flags[3]};
         const int j0 = d.j0, last = d.last;
@@ -470,7 +469,6 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       const int b = it & 1;
       const Info* const d = &s_info[it % kInfo];
       if (!wait(sfull(b), (it >> 1) & 1)) { ok = false; break; }
-      __syncwarp();
       tc_fence_after();
       uint32_t sr[64];
       tmem_ld32(tmem + b * kTile + lanes, *reinterpret_cast<uint32_t(*)[32]>(&sr[0]));
@@ -544,7 +542,6 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       // that of it - 2 or it - 1.)
       if (it > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
         if (!wait(pvdone, (it - 1) & 1)) { ok = false; break; }
-        __syncwarp();
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
