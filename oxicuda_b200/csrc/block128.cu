@@ -8,11 +8,11 @@
 //
 // A block of 128 columns is 16 lanes of 8 elements (one 16-byte load each), so its absmax is four shuffles: no shared
 // memory, and the scale is known without a second pass.  Statistics and scales are f32.  No element is divided (that would make the kernels
-// instruction-bound): v / scale is v * (max_val / absmax), the factor held as a sum of two floats, so that the quotient is rounded once.  In the
-// norm it is (r' gamma) * (max_val / absmax(r' gamma)): 1 / rms cancels and r' gamma is exact in f32 (two bf16).  Of 7.4 million codes of a
-// norm none then differs from the exact quotient's; with each step of the formula rounded 641 did.  In SwiGLU the hardware's exponential is
-// what is left: 2 codes in a million, as with the formula in f32 (a Newton step for the reciprocal and an exponent in two parts changed
-// neither that nor anything else but the time, 50 to 60 us for 2047 x 28672).
+// instruction-bound).  The norm's quotient is (r' gamma) * (max_val / absmax(r' gamma)): 1 / rms cancels, r' gamma is exact in f32 (two bf16),
+// and the factor is held as a sum of two floats, so that the quotient is rounded once: of 7.4 million codes none differs from the exact
+// quotient's; with each step of the formula rounded 641 did.  SwiGLU multiplies by the reciprocal of the scale, and makes the few elements that
+// come out next to a border between two codes again in 64 bits: 2047 x 28672 takes 58 us instead of 50, and no code above 2^-6 differs where
+// half a code in a million did.
 #include "common.cuh"
 
 namespace {
@@ -109,22 +109,18 @@ __device__ __forceinline__ NormScale norm_scale(float amax, float inv_rms, float
   }
   return n;
 }
-// The scales of the N blocks that a group of 16 lanes holds: lane k of the group makes the k'th (a division is some ten instructions), the
-// others get the factor hi + lo that takes its elements to codes.  `mine` is the scale that this lane made (k < N).
+// The scales of the N blocks that a group of 16 lanes holds: lane k of the group makes the k'th (a division and a reciprocal are some
+// twenty instructions each), the others get its reciprocal.  `mine` is the scale that this lane made (k < N).
 template <int N>
-__device__ __forceinline__ void block_scales(const float (&amax)[N], float max_val, float& mine, float (&fh)[N], float (&fl)[N]) {
+__device__ __forceinline__ void block_scales(const float (&amax)[N], float max_val, float& mine, float (&inv)[N]) {
   const int lane = threadIdx.x & 31, sub = lane & 15;
-  float a = amax[0], h, l = 0.0f;
+  float a = amax[0];
 #pragma unroll
   for (int k = 1; k < N; ++k) a = sub == k ? amax[k] : a;
   mine = block_scale(a, max_val);
-  if (a >= 0x1p-100f && a <= 0x1p100f) quotient(max_val, a, h, l);
-  else h = __frcp_rn(mine);
+  const float r = __frcp_rn(mine);
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    fh[k] = __shfl_sync(0xffffffffu, h, (lane & 16) | k);
-    fl[k] = __shfl_sync(0xffffffffu, l, (lane & 16) | k);
-  }
+  for (int k = 0; k < N; ++k) inv[k] = __shfl_sync(0xffffffffu, r, (lane & 16) | k);
 }
 __device__ __forceinline__ float block_sum(float v, float* sh) {
 #pragma unroll
@@ -329,6 +325,32 @@ __device__ __forceinline__ float silu_exact(float g) {
   return g * (g < 0.0f ? e : 1.0f) * __frcp_rn(1.0f + e);
 }
 
+// A quotient this near to the middle between two E4M3 codes may lie on its other side by the f32 arithmetic in front of it (2^-20 of itself; the
+// hardware's exponential and reciprocal, and some roundings, are off by about 2^-22 for gates of ordinary size).  Above 2^-6 the middles are the
+// floats whose 20 lowest bits are 0x80000, so the test is one multiply-add and a minimum.
+constexpr uint32_t kNear = 8u << 12;
+__device__ __forceinline__ uint32_t to_middle(float q) { return __float_as_uint(q) * 4096u + (0x80000000u + kNear); }   // below 2 kNear: near
+// The codes of a lane's 8 elements by the formula in 64 bits, for a whole warp (blocks of 16 lanes).
+__device__ __noinline__ uint2 swiglu_exact8(const __nv_bfloat16* gp, const __nv_bfloat16* up, bool live) {
+  double h[8], top = 0.0;
+#pragma unroll 1
+  for (int j = 0; j < 8; ++j) {
+    h[j] = 0.0;
+    if (live) {
+      const double g = (double)__bfloat162float(gp[j]);
+      h[j] = g * (double)__bfloat162float(up[j]) / (1.0 + exp(-g));
+    }
+    top = fmax(top, fabs(h[j]));
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const double f = top > 0.0 ? 448.0 / top : 1.0;
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2((float)(h[2 * j] * f), (float)(h[2 * j + 1] * f)), __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+}
+
 struct SwigluArgs {
   const __nv_bfloat16* gate; const __nv_bfloat16* up; int64_t rows, cols, ld; int fmt, rounding;
   float* scales; uint8_t* codes;
@@ -338,7 +360,7 @@ struct SwigluArgs {
 // 16 lanes per block of 128 columns, a warp two blocks; the blocks of all rows are one flat index space (below 2^31, so that its
 // division by the blocks of a row is a multiplication), two steps of it in flight per thread.
 template <int MODE>
-__global__ void __launch_bounds__(256) swiglu_block128_kernel(const SwigluArgs p) {
+__global__ void __launch_bounds__(256, 5) swiglu_block128_kernel(const SwigluArgs p) {
   b2q_pdl_entry();
   const uint32_t total = (uint32_t)p.rows * p.per_row, step = gridDim.x * 16;
   const int sub = threadIdx.x & 15;
@@ -362,7 +384,7 @@ __global__ void __launch_bounds__(256) swiglu_block128_kernel(const SwigluArgs p
       }
     }
     uint64_t h[2][4];
-    float amax[2], fh[2], fl[2], mine;
+    float amax[2], inv[2], mine;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       uint64_t g[4], u[4];
@@ -381,13 +403,23 @@ __global__ void __launch_bounds__(256) swiglu_block128_kernel(const SwigluArgs p
         amax[k] = max16(absmax8(h[k]));
       }
     }
-    block_scales<2>(amax, F.max_val, mine, fh, fl);
+    block_scales<2>(amax, F.max_val, mine, inv);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       if (sub == k && at[k] < total) p.scales[at[k]] = mine;
-      uint64_t q[4];
-      scale8(h[k], fh[k], fl[k], q);
-      if (live[k]) *reinterpret_cast<uint2*>(p.codes + row[k] * p.cols + col[k]) = encode8<MODE>(q, p.fmt, p.rounding, F);
+      const uint64_t inv2 = pair(inv[k], inv[k]), q[4] = {mul2(h[k][0], inv2), mul2(h[k][1], inv2), mul2(h[k][2], inv2), mul2(h[k][3], inv2)};
+      uint2 codes = encode8<MODE>(q, p.fmt, p.rounding, F);
+      if (MODE == kE4m3Rne) {
+        uint32_t near = 0xffffffffu;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) near = __vimin3_u32(near, to_middle(lo(q[j])), to_middle(hi(q[j])));
+        const bool sure = amax[k] >= 0x1p-100f && amax[k] <= 0x1p100f;             // of the whole block: its sums have neither over- nor underflowed
+        if (__any_sync(0xffffffffu, live[k] && sure && near < 2 * kNear)) {        // one warp in some two hundred
+          const uint2 exact = swiglu_exact8(p.gate + row[k] * p.ld + col[k], p.up + row[k] * p.ld + col[k], live[k]);
+          if (sure) codes = exact;
+        }
+      }
+      if (live[k]) *reinterpret_cast<uint2*>(p.codes + row[k] * p.cols + col[k]) = codes;
     }
   }
 }
@@ -434,7 +466,9 @@ extern "C" int32_t b2q_rms_norm_quantize_fp8_block128_bf16(b2q_handle h, const v
   const bool pdl = h->sw.chain_pdl != 0;
   const dim3 grid((unsigned)rows);
   if (cols % 8 == 0 && (align & 15) == 0 && chunks <= 4 * 1024) {
-    // few rows: one chunk per thread, the shortest chain; many rows: several chunks per thread, so that more CTAs share an SM
+    // Few rows: one chunk per thread, the shortest chain; many rows: several chunks per thread, so that more CTAs share an SM.  Measured with 1, 2
+    // and 4 chunks, us (taken: *): 7 x 4096 2.1*, 2.1, 2.9;  64 x 8192 2.8*, 2.6, 3.4;  512 x 8192 7.6, 6.6, 6.6*;  4096 x 8192 53, 45, 40*;
+    // 4096 x 4096 24, 22, 20*;  4096 x 2048 12.2, 10.3*, 11.1.
     int nch = chunks <= 1024 ? 1 : (chunks <= 2048 ? 2 : 4);
     if (rows >= 2 * (int64_t)h->sm_count && chunks > 128) nch = chunks <= 256 ? 2 : 4;
     const dim3 block((unsigned)(ceil_div64(ceil_div64(chunks, nch), 32) * 32));

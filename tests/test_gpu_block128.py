@@ -120,6 +120,22 @@ def test_norm_codes_are_those_of_the_exact_quotients(cuda):
     assert torch.equal(_values(codes)[clear], want[clear]) and clear.double().mean() > 0.999
 
 
+def test_swiglu_codes_are_those_of_the_exact_quotients(cuda):
+    """Elements next to a border between two codes are made again in 64 bits: above 2^-6 every code is the exact quotient's."""
+    from oxicuda_b200.quant import swiglu_quantize_fp8_block128
+    g = torch.Generator(device=cuda).manual_seed(5)
+    gate, up = [(1.5 * torch.randn(1000, 4096, device=cuda, generator=g)).to(torch.bfloat16) for _ in range(2)]
+    codes, _ = swiglu_quantize_fp8_block128(gate, up)
+    h = (gate.double() * up.double() / (1 + torch.exp(-gate.double()))).view(1000, 32, 128)
+    q = (h * (448.0 / h.abs().amax(dim=2, keepdim=True))).view(1000, 4096)
+    grid = torch.arange(127, dtype=torch.uint8, device=cuda).view(torch.float8_e4m3fn).double()
+    hi = torch.searchsorted(grid, q.abs()).clamp(1, 126)
+    mid = (grid[hi] + grid[hi - 1]) / 2
+    want = torch.where(q.abs() > mid, grid[hi], grid[hi - 1]) * torch.sign(q)
+    clear = ((q.abs() - mid).abs() > 2.0 ** -24 * q.abs()) & (q.abs() >= 2.0 ** -6)     # 2^-24: the rounding to f32 in front of the encoder
+    assert torch.equal(_values(codes)[clear], want[clear])
+
+
 def test_norm_of_non_finite_rows(cuda):
     """A row with a NaN is NaN throughout, a row with an infinity zeros and NaN (x / inf); the rows beside them are untouched."""
     from oxicuda_b200.kv_cache import rms_norm_quantize_fp8_block128
