@@ -248,6 +248,7 @@ class Handle:
     def __init__(self, device: int = 0):
         self._h = _H()
         self._stream = 0          # the stream the handle launches on (a new handle: the legacy default stream)
+        self.static_weights = True
         st = lib().b2q_create(C.byref(self._h), device)
         if st != OK:
             raise _ERRORS.get(st, B2qError)(st, "b2q_create failed (no CUDA device, or not an sm_100 GPU)")
@@ -277,6 +278,7 @@ class Handle:
     def set_static_weights(self, static_weights: bool):
         """False: weight operands may be produced by the kernel right before a call (see include/b2q.h)."""
         self.call("b2q_set_static_weights", 1 if static_weights else 0)
+        self.static_weights = bool(static_weights)
 
     def sm_version(self) -> int:
         v = _I()

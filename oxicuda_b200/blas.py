@@ -187,7 +187,9 @@ def gemm_fp8_block128(a: torch.Tensor, w: torch.Tensor, scale_a: torch.Tensor, s
                       out_dtype=torch.bfloat16, fmt: int = L.FP8_E4M3) -> torch.Tensor:
     """out[M,N] = sum over blocks b of 128 along K of scale_a[m,b] * scale_w[n/128,b] * (A[m,b] . W[n,b]): FP8 codes whose scales go
     per (row, 128 columns) of A [M,K] and per 128 x 128 block of W [N,K], f32 scales, f32 accumulation.  No counterpart in the
-    reference (its FP8 scales go per tensor)."""
+    reference (its FP8 scales go per tensor).  A `w` that is not contiguous is copied in every call.  Up to 128 rows of A the
+    weights may be fetched before the previous kernel of the stream has ended: where that kernel writes them, the handle's
+    set_static_weights(False) comes first."""
     if a.dim() != 2 or w.dim() != 2 or a.element_size() != 1 or w.element_size() != 1:
         raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, "gemm_fp8_block128 takes two matrices of 8-bit codes")
     M, K = a.shape
@@ -205,9 +207,17 @@ def gemm_fp8_block128(a: torch.Tensor, w: torch.Tensor, scale_a: torch.Tensor, s
     elif tuple(out.shape) != (M, N) or out.dtype not in (torch.bfloat16, torch.float32) or not out.is_contiguous():
         raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, "gemm_fp8_block128: out must be a contiguous bf16 or f32 tensor [M, N]")
     L.require_cuda("gemm_fp8_block128", a=a, w=w, scale_a=scale_a, scale_w=scale_w, out=out)
+    h = default_handle()
+    copied = not w.is_contiguous() and h.static_weights    # the copy may be the kernel right before the product, which must not fetch weights ahead of it
     a, w, scale_a, scale_w = a.contiguous(), w.contiguous(), scale_a.contiguous(), scale_w.contiguous()
-    default_handle().call("b2q_gemm_fp8_block128", a.data_ptr(), w.data_ptr(), M, N, K, fmt, scale_a.data_ptr(), scale_w.data_ptr(), out.data_ptr(),
-                          L.OUT_BF16 if out.dtype == torch.bfloat16 else L.OUT_F32)
+    if copied:
+        h.set_static_weights(False)
+    try:
+        h.call("b2q_gemm_fp8_block128", a.data_ptr(), w.data_ptr(), M, N, K, fmt, scale_a.data_ptr(), scale_w.data_ptr(), out.data_ptr(),
+               L.OUT_BF16 if out.dtype == torch.bfloat16 else L.OUT_F32)
+    finally:
+        if copied:
+            h.set_static_weights(True)
     return out
 
 

@@ -1,0 +1,49 @@
+"""GPU: block-128 calls with operands as programs hold them: strided weights, weights written right before the call.  Tolerances as in
+test_gpu_block128.py."""
+import pytest
+import torch
+
+from tests.test_gpu_block128 import _check_product, _operands
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("M", [1, 17, 60, 128, 200])
+def test_strided_weights(cuda, M):
+    """A transposed weight and a column shard of a wider one give the bits of their contiguous copies, with new weights in every call."""
+    from oxicuda_b200.blas import gemm_fp8_block128
+    N, K = 640, 2048
+    for seed in range(4):
+        a, w, sa, sw = _operands(cuda, M, N, K, 0, 100 * M + seed)
+        want = gemm_fp8_block128(a, w, sa, sw)
+        _check_product(a, w, sa, sw, want)
+        torch.cuda.synchronize()
+        turned = torch.empty(K, N, dtype=torch.uint8, device=cuda)
+        turned.copy_(w.t())
+        assert torch.equal(gemm_fp8_block128(a, turned.t(), sa, sw), want)
+        wide = torch.full((N, 3 * K), 0x7F, dtype=torch.uint8, device=cuda)
+        wide[:, K: 2 * K] = w
+        assert torch.equal(gemm_fp8_block128(a, wide[:, K: 2 * K], sa, sw), want)
+
+
+@pytest.mark.parametrize("M", [1, 40, 128])
+def test_weights_written_right_before_the_product(cuda, M):
+    """With static_weights off the few-token product reads nothing before the kernel that writes its weights has completed."""
+    from oxicuda_b200 import _lib as L
+    from oxicuda_b200.blas import gemm_fp8_block128
+    h = L.default_handle()
+    N, K = 8192, 2048
+    sets = [_operands(cuda, M, N, K, 0, 7 * M + i) for i in range(3)]
+    want = [gemm_fp8_block128(*s) for s in sets]
+    for s, x in zip(sets, want):
+        _check_product(*s, x)
+    torch.cuda.synchronize()
+    w = torch.full((N, K), 0x7F, dtype=torch.uint8, device=cuda)
+    h.set_static_weights(False)
+    try:
+        for (a, new, sa, sw), x in zip(sets, want):
+            w.copy_(new)                                            # same stream, no synchronisation
+            assert torch.equal(gemm_fp8_block128(a, w, sa, sw), x)
+    finally:
+        h.set_static_weights(True)
+    h.check()
