@@ -18,7 +18,7 @@ namespace cg = cooperative_groups;
 namespace b128few {
 
 constexpr int ROWS = 128, BK = 128;
-constexpr uint64_t kWaitLimitNs = 10000000000ull;    // the first waits may begin while the previous kernel of the stream still runs
+constexpr uint64_t kWaitLimitNs = 500000000ull;      // counted from the previous kernel's end
 
 template <int NB> struct Cfg {           // NB: accumulator columns = padded tokens
   static constexpr int kBytesW = ROWS * BK, kBytesX = NB * BK, kStageBytes = kBytesW + kBytesX;
@@ -107,18 +107,19 @@ gemm_block128_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, s_tmem_base, 0);
   volatile int* abort_flag = &s_abort;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // Every thread waits for the previous kernel here: it may still be reading what this one stores, and no bounded wait counts its time.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   constexpr int COLS = C::kCols, NACC = COLS / 2;
   const int col0 = warp >= 4 ? ((warp >> 2) - 1) * COLS : 0;           // the epilogue thread's tokens
   uint64_t acc[NACC];
 #pragma unroll
   for (int j = 0; j < NACC; ++j) acc[j] = 0;
+  bool ok = true;                                      // false: this warp has given up a wait
 
   if (warp == 0) {
-    // ---------------- TMA: weights, and the activations behind the previous kernel (rows past the last token are zero-filled) ----------------
+    // ---------------- TMA: weights and activations (rows past the last token are zero-filled) ----------------
     if (lane == 0) {
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-      bool ok = true;
       for (int it = 0; it < total; ++it) {
         const int s = it % kStages, x = (k_begin + it) * BK;
         const uint32_t at = base + s * C::kStageBytes;
@@ -136,7 +137,6 @@ gemm_block128_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer: one accumulator per block of K; the warp stays together and elects a lane (descriptors in uniform registers) ----------------
-    bool ok = true;
     for (int it = 0; it < total; ++it) {
       const int s = it % kStages, b = it % kBuf;
       ok = warp_wait(tempty_bar(b), ((it / kBuf) & 1) ^ 1, abort_flag) && warp_wait(full_bar(s), (it / kStages) & 1, abort_flag);
@@ -161,7 +161,6 @@ gemm_block128_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
     }
   } else if (warp < 4) {
     // ---------------- scales: scale_a * scale_w of each token, four blocks of K at a time ----------------
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int PER = NB > 64 ? 2 : 1;
     const int t0 = (int)threadIdx.x - 64;
     const float* sw = p.sw + (int64_t)tile * p.kb;
@@ -194,8 +193,8 @@ gemm_block128_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     for (int it = 0, i = 0; it < total; ++it) {
       const int b = it % kBuf, slot = i % C::kSlots;
-      if ((it & 3) == 0 && !warp_wait(sfull_bar(slot), (i / C::kSlots) & 1, abort_flag)) break;
-      if (!warp_wait(tfull_bar(b), (it / kBuf) & 1, abort_flag)) break;
+      ok = ((it & 3) != 0 || warp_wait(sfull_bar(slot), (i / C::kSlots) & 1, abort_flag)) && warp_wait(tfull_bar(b), (it / kBuf) & 1, abort_flag);
+      if (!ok) break;
       __syncwarp();
       tc_fence_after();
       const ulonglong2* c = reinterpret_cast<const ulonglong2*>(s_scale + (slot * 4 + (it & 3)) * NB + col0);   // every lane reads the same
@@ -232,7 +231,7 @@ gemm_block128_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
     else reinterpret_cast<float*>(p.out)[(int64_t)t * p.N + at] = v;
   };
   if (split == 1) {
-    if (row >= 0 && n < p.N) {
+    if (row >= 0 && n < p.N && ok) {
 #pragma unroll
       for (int t = 0; t < COLS; ++t)
         if (col0 + t < p.tokens) store(col0 + t, n, __uint_as_float((uint32_t)(acc[t / 2] >> (32 * (t & 1)))));
