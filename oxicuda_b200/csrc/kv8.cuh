@@ -86,6 +86,27 @@ __device__ __forceinline__ int div_group(const AttendArgs& p, int x) { return (i
 
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(min(127, max(-126, e)) + 127) << 23); }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// The unit of the outputs, 2^R.  Value codes are multiplied as they are stored, so a page's scale 2^lv enters with the f16 weights: a weight is
+// p * 2^x, x = X + lv - R (X is the attention kernel's own), and outputs are summed in units of 2^(R - X).  R follows the pages: up when one lies above
+// it (f16 must hold the weight), down when one lies more than 2^kSpan below it, but by 2^kDrop at most below the largest unit so far.  What was
+// summed in that unit is below 2^15 * 448 * 2^31 keys < 2^55 of it, so it stays below 2^119 in the smaller one.
+constexpr int kNone = -1000;                     // R before the first page
+constexpr int kSpan = 8, kDrop = 64;
+// The weights of a page so far below R that f16 holds none of them: x is not less than this, so that their sum in f32 still counts them.
+constexpr int kLeast = -40;
+// what outputs are multiplied by when R moves: 2^(from - to), exact down to 2^-149 and 0 below (R may rise by 2^171)
+__device__ __forceinline__ float move_unit(int from, int to) {
+  const int d = from - to;
+  return d >= -126 ? pow2i(d) : d >= -149 ? __uint_as_float(1u << (d + 149)) : 0.0f;
+}
+// R for pages whose largest value scale is 2^lead; `top` is the largest R so far.  Returns what outputs are to be multiplied by.
+__device__ __forceinline__ float next_unit(int& R, int& top, int lead, int room) {
+  if (lead <= R && lead >= R - kSpan) return 1.0f;
+  const int was = R;
+  R = lead > R ? lead + room : max(lead + room, top - kDrop);
+  top = max(top, R);
+  return was == kNone ? 1.0f : move_unit(was, R);
+}
 __device__ __forceinline__ float pow2_byte(uint32_t e8m0) { return e8m0_to_f32_dev(e8m0); }
 
 }  // namespace kv8

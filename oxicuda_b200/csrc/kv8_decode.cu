@@ -16,8 +16,8 @@
 // barrier between them.  Warps and the CTAs of a cluster (tiles dealt round) are joined once at the end, through shared and distributed
 // shared memory: no workspace, one launch, and a result that does not depend on timing.
 // The value scale is a power of two 2^lv per page: weights enter as p * 2^(15 + lv - R) and the outputs are kept in units of
-// 2^(R - 15), R following the pages' scales, so the weights keep their precision whatever the pages' sizes are; pages of one tile
-// whose scales lie more than 2^8 apart are multiplied one after the other.
+// 2^(R - 15), R following the pages' scales (next_unit in kv8.cuh); pages of one tile whose scales lie more than 2^8 apart are multiplied
+// one after the other.
 // Keys behind the last visible one are masked and their value rows zeroed before they are multiplied, so stale codes cannot reach a
 // result; a page that the table does not name is neither read nor counted.
 // Measured: 32 sequences x 8200 keys (32 heads of 128 channels over 8 kv heads) 90 us, 4.5 TB/s of cache (pages of 16: 94 us); the same copies
@@ -42,8 +42,6 @@ template <int D> struct Ring {
   static_assert(kStages % (kWarps / 2) == 0, "a stage belongs to one pair of warps, which cannot run a phase ahead of its own");
   static constexpr int kSmem = kStages * kStage + kStages * 32 + 1024;
 };
-constexpr int kNone = -1000;                     // R of a warp that has seen no page
-constexpr int kSpan = 8;                         // value scales that share a product differ by at most 2^kSpan
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -144,7 +142,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 
   float o[RB][MT][4];
   float m[RB][2], l[RB][2];
-  int R = kNone;
+  int R = kNone, top = kNone;                    // unit of o, the largest so far
 #pragma unroll
   for (int x = 0; x < RB; ++x) {
 #pragma unroll
@@ -387,10 +385,9 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         float alpha[RB][2];
         uint32_t pb[RB][4];
         if (clear) {
-          const int lead = max(lv[0], lv[1]), was = R == kNone ? lead : R;
-          R = lead > was || lead < was - kSpan ? lead : was;
-          const float kf[2] = {pow2_byte(sc[0] & 0xFF), pow2_byte(sc[1] & 0xFF)}, move = pow2i(was - R);
-          const float down[2] = {pow2i(R - lv[0] - 15), pow2i(R - lv[1] - 15)}, shift[2] = {(float)(15 + lv[0] - R), (float)(15 + lv[1] - R)};
+          const float move = next_unit(R, top, max(lv[0], lv[1]), 0), kf[2] = {pow2_byte(sc[0] & 0xFF), pow2_byte(sc[1] & 0xFF)};
+          const int up[2] = {max(15 + lv[0] - R, kLeast), max(15 + lv[1] - R, kLeast)};
+          const float down[2] = {pow2i(-up[0]), pow2i(-up[1])}, shift[2] = {(float)up[0], (float)up[1]};
 #pragma unroll
           for (int x = 0; x < RB; ++x) {
             float w[4][2];
@@ -435,9 +432,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           while (rem) {
             const int lead = rem == 3 ? max(lv[0], lv[1]) : rem == 1 ? lv[0] : lv[1];
             const unsigned take = rem & ((lv[0] >= lead - kSpan ? 1u : 0u) | (lv[1] >= lead - kSpan ? 2u : 0u));
-            const int was = R == kNone ? lead : R;
-            R = lead > was || lead < was - kSpan ? lead : was;
-            const float move = pow2i(was - R), up[2] = {take & 1 ? pow2i(15 + lv[0] - R) : 0.0f, take & 2 ? pow2i(15 + lv[1] - R) : 0.0f};
+            const float move = next_unit(R, top, lead, 0), up[2] = {take & 1 ? pow2i(15 + lv[0] - R) : 0.0f, take & 2 ? pow2i(15 + lv[1] - R) : 0.0f};
 #pragma unroll
             for (int x = 0; x < RB; ++x) {
               alpha[x][0] *= move; alpha[x][1] *= move;
@@ -479,8 +474,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   auto finish = [&](int rr, int cc, const float4 acc, float mm, float ll, int unit_exp) {
     const int hd = head0 + rr, tk = hd / p.group;
     const int64_t orow = (int64_t)(r.r0 + token0 + tk) * (t.n_kv_heads * p.group) + head * p.group + (hd - tk * p.group);
-    const float k = (ll == 0.0f ? 0.0f : __frcp_rn(ll)), up = unit_exp == kNone ? 0.0f : pow2i(unit_exp - 15);
-    const __nv_bfloat162 y0 = __floats2bfloat162_rn(acc.x * k * up, acc.y * k * up), y1 = __floats2bfloat162_rn(acc.z * k * up, acc.w * k * up);
+    const float k = (ll == 0.0f ? 0.0f : __frcp_rn(ll)) * (unit_exp == kNone ? 0.0f : pow2i(unit_exp - 15));
+    const __nv_bfloat162 y0 = __floats2bfloat162_rn(acc.x * k, acc.y * k), y1 = __floats2bfloat162_rn(acc.z * k, acc.w * k);
     uint2 pk;
     pk.x = *reinterpret_cast<const uint32_t*>(&y0); pk.y = *reinterpret_cast<const uint32_t*>(&y1);
     *reinterpret_cast<uint2*>(p.out + orow * D + cc) = pk;
@@ -498,7 +493,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float a = ex2(s_m[w][rr] - b), fo = a * (s_r[w] == kNone ? 0.0f : pow2i(s_r[w] - cr));
+      const float a = ex2(s_m[w][rr] - b), fo = a * (s_r[w] == kNone ? 0.0f : move_unit(s_r[w], cr));
       ll += a * s_l[w][rr];
       const float4 x = *reinterpret_cast<const float4*>(&s_o[w][rr][cc]);
       acc.x += fo * x.x; acc.y += fo * x.y; acc.z += fo * x.z; acc.w += fo * x.w;
@@ -525,7 +520,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       for (int c = 0; c < split; ++c) {
         const float a = ex2(*cluster.map_shared_rank(&s_cm[rr], c) - b);
         const int rc = *cluster.map_shared_rank(&s_cr, c);
-        const float fo = a * (rc == kNone ? 0.0f : pow2i(rc - tr));
+        const float fo = a * (rc == kNone ? 0.0f : move_unit(rc, tr));
         ll += a * *cluster.map_shared_rank(&s_cl[rr], c);
         const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(&s_o[0][rr][cc], c));
         acc.x += fo * x.x; acc.y += fo * x.y; acc.z += fo * x.z; acc.w += fo * x.w;

@@ -40,9 +40,7 @@ constexpr int kRows = 128, kTile = 64;
 constexpr int kThreads = 256;
 constexpr int kRegsFirst = 80, kRegsSoft = 176;  // of 128 a thread at launch: 128 * 80 + 128 * 176 = 256 * 128
 constexpr int kKStages = 3, kVStages = 2, kInfo = 8;   // tiles in flight; tile descriptions (a tile is read at most 5 behind the newest)
-constexpr int kSpan = 8;                         // value scales that share a tile differ by at most 2^kSpan
 constexpr int kRoom = 2;                         // R is set that far above a scale, so that pages a little larger do not move it again
-constexpr int kNone = -1000;
 constexpr float kSlack = 6.0f;                   // 2^(8 + 6) is well inside f16
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 constexpr int kGridY = 32768;                    // row tiles: blockIdx.y, and z beyond that
@@ -278,7 +276,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
       };
       bool ok = true;
-      int R = kNone, it = 0;                        // tiles issued: a tile is walked once per group of pages whose value scales are alike
+      int R = kNone, top = kNone, it = 0;           // it: tiles issued: a tile is walked once per group of pages whose value scales are alike
       fetch(0);
       for (int i0 = 0; i0 < tiles && ok; i0 += 32) {
         int cp[SUBS];
@@ -310,9 +308,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 #pragma unroll
             for (int e = 0; e < SUBS; ++e) take |= (rem >> e & 1) && (int)(fl[e] >> 8 & 0xFF) - 127 >= lead - kSpan ? 1u << e : 0u;
             rem &= ~take;
-            const int was = R == kNone ? lead + kRoom : R;
-            const float move = R == kNone ? 1.0f : 0.0f;
-            R = lead == kNone ? R : lead > was || lead < was - kSpan ? lead + kRoom : was;
+            const float move = lead == kNone ? 1.0f : next_unit(R, top, lead, kRoom);
             float kf[SUBS], up[SUBS], down[SUBS];
             uint32_t flag[SUBS];
 #pragma unroll
@@ -320,8 +316,9 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
               const int lv = (int)(fl[e] >> 8 & 0xFF) - 127;
               flag[e] = (fl[e] & kThere) | (take >> e & 1 ? kTaken : 0u);
               kf[e] = pow2_byte(fl[e] & 0xFF);
-              up[e] = (float)(8 + lv - R);
-              down[e] = pow2i(R - lv - 8);
+              const int x = max(8 + lv - R, kLeast);
+              up[e] = (float)x;
+              down[e] = pow2i(-x);
             }
             constexpr int A2 = SUBS == 4 ? 1 : 0, C2 = SUBS / 2, D2 = SUBS - 1;   // the pages of keys 16 .. 31, 32 .. 47, 48 .. 63
             const int s = it % kKStages, v = it % kVStages;
@@ -333,7 +330,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
               *reinterpret_cast<float4*>(d->kf) = make_float4(kf[0], kf[A2], kf[C2], kf[D2]);
               *reinterpret_cast<float4*>(d->up) = make_float4(up[0], up[A2], up[C2], up[D2]);
               *reinterpret_cast<float4*>(d->down) = make_float4(down[0], down[A2], down[C2], down[D2]);
-              *reinterpret_cast<int4*>(&d->j0) = make_int4(j, i0 + i == tiles - 1 && !rem, R, __float_as_int(move != 0.0f ? move : pow2i(was - R)));
+              *reinterpret_cast<int4*>(&d->j0) = make_int4(j, i0 + i == tiles - 1 && !rem, R, __float_as_int(move));
               mbar_expect_tx(kfull(s), (uint32_t)(there * rows_each * D));
 #pragma unroll
               for (int e = 0; e < SUBS; ++e)
@@ -565,7 +562,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     // a row that sees no key has l = 0: zeros and -inf.  A query that holds an infinity or a NaN has l = NaN and stays NaN.
     if (split == 1) {
       const int64_t orow = (int64_t)(r.r0 + token) * (t.n_kv_heads * p.group) + qhead;
-      const float inv = l == 0.0f ? 0.0f : __frcp_rn(l), up = R == kNone ? 0.0f : pow2i(R - 8);
+      const float inv = (l == 0.0f ? 0.0f : __frcp_rn(l)) * (R == kNone ? 0.0f : pow2i(R - 8));
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
@@ -578,7 +575,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[j + 2 * i]) * inv * up, __uint_as_float(o[j + 2 * i + 1]) * inv * up);
+              const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[j + 2 * i]) * inv, __uint_as_float(o[j + 2 * i + 1]) * inv);
               w[i] = *reinterpret_cast<const uint32_t*>(&h);
             }
             y[j / 8] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -618,15 +615,15 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       for (int c = 0; c < split; ++c) {
         const float a = ex2(*cluster.map_shared_rank(&s_m[row], c) - back);
         const int rc = *cluster.map_shared_rank(&s_r[row], c);
-        const float fo = a * (rc == kNone ? 0.0f : pow2i(rc - rr));
+        const float fo = a * (rc == kNone ? 0.0f : move_unit(rc, rr));
         ll += a * *cluster.map_shared_rank(&s_l[row], c);
         const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(smem + row * (D * 4) + ((u ^ (row & 7)) << 4), c));
         acc.x += fo * x.x; acc.y += fo * x.y; acc.z += fo * x.z; acc.w += fo * x.w;
       }
       const int tk = div_group(p, head0 + row), hd = head * p.group + head0 + row - tk * p.group;
       const int64_t orow = (int64_t)(r.r0 + token0 + tk) * (t.n_kv_heads * p.group) + hd;
-      const float inv = ll == 0.0f ? 0.0f : __frcp_rn(ll), up = rr == kNone ? 0.0f : pow2i(rr - 8);
-      const __nv_bfloat162 y0 = __floats2bfloat162_rn(acc.x * inv * up, acc.y * inv * up), y1 = __floats2bfloat162_rn(acc.z * inv * up, acc.w * inv * up);
+      const float inv = (ll == 0.0f ? 0.0f : __frcp_rn(ll)) * (rr == kNone ? 0.0f : pow2i(rr - 8));
+      const __nv_bfloat162 y0 = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), y1 = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
       uint2 pk;
       pk.x = *reinterpret_cast<const uint32_t*>(&y0); pk.y = *reinterpret_cast<const uint32_t*>(&y1);
       *reinterpret_cast<uint2*>(p.out + orow * D + 4 * u) = pk;
