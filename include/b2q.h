@@ -222,7 +222,9 @@ int32_t b2q_kv8_append_bf16(b2q_handle h, const void* k, const void* v, int64_t 
  * logarithm of the softmax denominators.  A row that sees no key gives zeros and -inf.  Table entries of pages that no row's window
  * reaches are not looked at.  A query that holds an infinity or a NaN makes its own row NaN; the codes of cached tokens are taken to be
  * finite, as b2q_kv8_append_bf16 writes them (a slot that holds no token may hold anything).  Scores, maxima, sums and outputs are held in
- * f32; a query element is off by at most 2^-17 of its row's largest, a softmax weight by 2^-9 of itself. */
+ * f32; a query element is off by at most 2^-17 of its row's largest, a softmax weight by 2^-11 of itself or by 2^-25 of the row's largest weight.
+ * That holds while the value scales of a sequence's pages lie within 2^64 of one another.  Beyond that the values of smaller pages lose bits of their
+ * weights, and count as zeros from 2^90 below the largest on; outputs stay finite, and the log-sum-exp counts every key. */
 int32_t b2q_kv8_attention_bf16(b2q_handle h, const void* q, int64_t ld_q, int64_t tokens, int64_t n_heads, const int32_t* q_starts,
                                const int32_t* seq_lens, const int32_t* block_tables, int64_t seqs, int64_t table_width, int64_t num_pages,
                                int64_t page_size, int64_t n_kv_heads, int64_t head_dim, const uint8_t* k_codes, const uint8_t* v_codes,

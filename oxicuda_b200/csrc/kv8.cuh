@@ -88,8 +88,9 @@ __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 // The unit of the outputs, 2^R.  Value codes are multiplied as they are stored, so a page's scale 2^lv enters with the f16 weights: a weight is
 // p * 2^x, x = X + lv - R (X is the attention kernel's own), and outputs are summed in units of 2^(R - X).  R follows the pages: up when one lies above
-// it (f16 must hold the weight), down when one lies more than 2^kSpan below it, but by 2^kDrop at most below the largest unit so far.  What was
-// summed in that unit is below 2^15 * 448 * 2^31 keys < 2^55 of it, so it stays below 2^119 in the smaller one.
+// it (f16 must hold the weight), down when one lies more than 2^kSpan below it (x is X - kSpan at least: a weight is off by 2^-11 of itself or by
+// 2^-(25 + x)), but by 2^kDrop at most below the largest unit so far.  What was summed in that unit is below 2^15 * 448 * 2^31 keys < 2^55 of it,
+// so it stays below 2^119 in the smaller one.
 constexpr int kNone = -1000;                     // R before the first page
 constexpr int kSpan = 8, kDrop = 64;
 // The weights of a page so far below R that f16 holds none of them: x is not less than this, so that their sum in f32 still counts them.
@@ -99,9 +100,10 @@ __device__ __forceinline__ float move_unit(int from, int to) {
   const int d = from - to;
   return d >= -126 ? pow2i(d) : d >= -149 ? __uint_as_float(1u << (d + 149)) : 0.0f;
 }
-// R for pages whose largest value scale is 2^lead; `top` is the largest R so far.  Returns what outputs are to be multiplied by.
-__device__ __forceinline__ float next_unit(int& R, int& top, int lead, int room) {
-  if (lead <= R && lead >= R - kSpan) return 1.0f;
+// R for pages whose value scales lie from 2^least to 2^lead, lead + room - least at most kSpan; `top` is the largest R so far.  Returns what outputs are
+// to be multiplied by.
+__device__ __forceinline__ float next_unit(int& R, int& top, int lead, int least, int room) {
+  if (lead <= R && least >= R - kSpan) return 1.0f;
   const int was = R;
   R = lead > R ? lead + room : max(lead + room, top - kDrop);
   top = max(top, R);

@@ -8,7 +8,7 @@
 //   scores^T  [16 keys x 8 rows] = K [16 x D] . Q^T;      outputs^T [16 channels x 8 rows] = V^T [16 x keys] . P^T.
 // An E4M3 code is exact in f16 (one conversion instruction for two).  Q enters as f16 after a power of two has brought its row's
 // largest element into [2^14, 2^15): a bf16 has 8 significant bits and f16 has 11, so it is exact but for elements below 2^-28 of that
-// largest.  The weights enter as p * 2^15 rounded to f16: off by 2^-12 of themselves, or of 2^-29 below the normal range.
+// largest.  The weights enter as p * 2^7 to p * 2^15 rounded to f16: off by 2^-11 of themselves, or by 2^-32 of the row's largest.
 // Channels are dealt to lanes so that a lane's operands are 16 neighbouring bytes of a row (both products sum over, or are independent
 // of, the order of channels); 8 x 8 tiles of P are transposed between lanes by movmatrix, pairs of keys of V by byte permutations.
 // One warp brings tiles of 64 keys into a ring of shared memory by TMA (it alone walks the block table, a batch of tiles ahead); three
@@ -385,7 +385,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         float alpha[RB][2];
         uint32_t pb[RB][4];
         if (clear) {
-          const float move = next_unit(R, top, max(lv[0], lv[1]), 0), kf[2] = {pow2_byte(sc[0] & 0xFF), pow2_byte(sc[1] & 0xFF)};
+          const float move = next_unit(R, top, max(lv[0], lv[1]), min(lv[0], lv[1]), 0), kf[2] = {pow2_byte(sc[0] & 0xFF), pow2_byte(sc[1] & 0xFF)};
           const int up[2] = {max(15 + lv[0] - R, kLeast), max(15 + lv[1] - R, kLeast)};
           const float down[2] = {pow2i(-up[0]), pow2i(-up[1])}, shift[2] = {(float)up[0], (float)up[1]};
 #pragma unroll
@@ -432,7 +432,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           while (rem) {
             const int lead = rem == 3 ? max(lv[0], lv[1]) : rem == 1 ? lv[0] : lv[1];
             const unsigned take = rem & ((lv[0] >= lead - kSpan ? 1u : 0u) | (lv[1] >= lead - kSpan ? 2u : 0u));
-            const float move = next_unit(R, top, lead, 0), up[2] = {take & 1 ? pow2i(15 + lv[0] - R) : 0.0f, take & 2 ? pow2i(15 + lv[1] - R) : 0.0f};
+            const float move = next_unit(R, top, lead, take == 3 ? min(lv[0], lv[1]) : take == 1 ? lv[0] : lv[1], 0), up[2] = {take & 1 ? pow2i(15 + lv[0] - R) : 0.0f, take & 2 ? pow2i(15 + lv[1] - R) : 0.0f};
 #pragma unroll
             for (int x = 0; x < RB; ++x) {
               alpha[x][0] *= move; alpha[x][1] *= move;

@@ -8,7 +8,7 @@
 // cost what one bf16 product costs, and the split is made once per row.
 // P V multiplies in f16 (kind::f16): two warps turn each value tile into f16 (exact, one conversion for 128 rows of P, where
 // splitting P into E4M3 terms costs every row four instructions per pair of weights), P goes back into the TMEM columns of its S as the
-// A operand.  A weight is held as p * 2^8 and is off by 2^-12 of itself, or of 2^-22 below the normal range of f16.
+// A operand.  A weight is held as p * 2^x, x from 0 to 8 (6 for most pages), and is off by 2^-11 of itself, or by 2^-25 of the row's largest (2^-31).
 // Work per 64 keys and CTA: 640 clocks of tensor core (Q K^T at N = 64 reads 1.5 x the shared memory that its rate allows, P V at N = D
 // runs at rate), 512 of exponentials and 120 KB of shared memory traffic (48 for Q K^T, 16 for P V, 40 to convert the values, 16 to bring the
 // tiles in), 940 clocks: two CTAs share an SM, so that one multiplies while the other exponentiates.
@@ -17,8 +17,8 @@
 // three quarters of Q K^T 10 %: shared memory bounds it, with the products' latency on top in short rows.
 // The running maximum is followed lazily: it moves only when a score exceeds it by more than 2^kSlack (f16 has the range), so O is rescaled
 // (a round trip through registers) once or twice per row and not per tile.  The value scale of a page is a power of two 2^lv: weights
-// enter as p * 2^(8 + lv - R) and O is in units of 2^(R - 8); a tile whose pages differ by more than 2^kSpan is walked once per group
-// of alike pages, the others masked.
+// enter as p * 2^(8 + lv - R) and O is in units of 2^(R - 8), R following the pages (next_unit in kv8.cuh); a tile whose pages differ by more
+// than 2^(kSpan - kRoom) is walked once per group of alike pages, the others masked.
 // Few row tiles: `split` CTAs of a cluster take every split'th key tile of the same rows and are joined through distributed shared memory.
 // Warps 1 to 7 turn the query rows into E4M3 terms; then warp 0 walks the block table, issues the copies and describes each tile to the others,
 // warp 1 issues the products, warps 2 and 3 convert values, warps 4 to 7 are the softmax (a thread to a row).
@@ -301,14 +301,17 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           bool once = true;                         // a tile without any page is walked too: its rows see none of it
           while ((rem || once) && ok) {
             once = false;
-            int lead = kNone;
+            int lead = kNone, least = 1000;
             unsigned take = 0;
 #pragma unroll
             for (int e = 0; e < SUBS; ++e) if (rem >> e & 1) lead = max(lead, (int)(fl[e] >> 8 & 0xFF) - 127);
 #pragma unroll
-            for (int e = 0; e < SUBS; ++e) take |= (rem >> e & 1) && (int)(fl[e] >> 8 & 0xFF) - 127 >= lead - kSpan ? 1u << e : 0u;
+            for (int e = 0; e < SUBS; ++e) {
+              const int lv = (int)(fl[e] >> 8 & 0xFF) - 127;
+              if ((rem >> e & 1) && lv >= lead + kRoom - kSpan) { take |= 1u << e; least = min(least, lv); }
+            }
             rem &= ~take;
-            const float move = lead == kNone ? 1.0f : next_unit(R, top, lead, kRoom);
+            const float move = lead == kNone ? 1.0f : next_unit(R, top, lead, least, kRoom);
             float kf[SUBS], up[SUBS], down[SUBS];
             uint32_t flag[SUBS];
 #pragma unroll

@@ -4,7 +4,7 @@ Tolerance of an output, with l = sum exp(s - max), p the weights, v = 2^lv c, an
   2^-8 |o|                                   the result's rounding to bf16
   (2^-11 + 3 delta) sum p |v|                a weight's rounding to f16, and what the query's rounding moves it (as in test_gpu_kv8.py)
   sum |c| 2^-25 max(2^(lv + 8), 2^(TOP - 70)) / l   weights below the normal range of f16: the unit of the outputs is 2^(R - 8) at most, R at most
-                                             lv + 16, or TOP + 2 - 64 where it may not follow
+                                             lv + 8 (16 are allowed here; the last test is closer), or TOP + 2 - 64 where it may not follow
   2^(TOP - 142) / l                          what was summed before the unit rose to 2^(TOP + 2 - 8), below f32's smallest number"""
 import math
 
@@ -93,3 +93,35 @@ def test_rows_that_do_not_see_the_large_pages_behind_them(cuda, ps, d, new, low,
     pages = max(4, 512 // ps)
     _run(cuda, [low] * (pages - 1) + [high], ps, d, new, low + high + ps, group=1 if new == 2 else 4)
     _run(cuda, [low] * (pages - 1) + [high] * 3, ps, d, min(new, 3 * ps), high + ps)
+
+
+@pytest.mark.parametrize("new,top,lead,low,score", [(1, 8, 0, -8, 13.5958), (32, 16, 10, 2, 8.7437)])
+def test_small_weights_on_pages_of_a_smaller_scale(cuda, new, top, lead, low, score):
+    """Many keys of one small weight on the smallest of pages that are multiplied together: e^-13.6 and e^-8.7 lie 0.45 steps above a number of f16's
+    subnormal range if they enter as p * 2^-1 and p * 2^-8, 4 % off.  All of the output comes from them."""
+    from oxicuda_b200.kv_cache import PagedFp8KvCache
+    ps, d, front, pairs = 16, 128, 96, 48
+    exps = [top] * front + [lead, low] * pairs
+    g = torch.Generator(device=cuda).manual_seed(new)
+    n = len(exps)
+    k = torch.zeros(n, 1, ps, d, dtype=torch.uint8, device=cuda)
+    k[front:, :, :, 0] = 0xB8                              # -1: these keys score -score, those in front 0
+    v = (100 + 50 * torch.rand(n, 1, ps, d, device=cuda, generator=g)).to(torch.float8_e4m3fn).view(torch.uint8)
+    v[:front] = 0
+    v[front::2] = 0
+    scales = (torch.tensor(exps, device=cuda) + 127).to(torch.uint8)[:, None].contiguous()
+    cache = PagedFp8KvCache(k, v, torch.full_like(scales, 127), scales)
+    q = torch.zeros(new, 4, d, dtype=torch.bfloat16, device=cuda)
+    q[..., 0] = 1
+    keys = n * ps
+    starts = None if new == 1 else torch.tensor([0, new], dtype=torch.int32, device=cuda)
+    out = cache.attend(q, torch.tensor([keys], dtype=torch.int32, device=cuda), torch.arange(n, dtype=torch.int32, device=cuda)[None].contiguous(), q_starts=starts,
+                       scale=score)
+    value = (v.view(torch.float8_e4m3fn).double() * torch.exp2(torch.tensor(exps, device=cuda).double())[:, None, None, None]).view(keys, d)
+    s = torch.where(torch.arange(keys, device=cuda) < front * ps, 0.0, -score).double()
+    see = torch.arange(keys, device=cuda)[None] <= (keys - new + torch.arange(new, device=cuda))[:, None]
+    p = torch.exp(s)[None] * see
+    want = ((p @ value) / p.sum(dim=1, keepdim=True))[:, None].expand(new, 4, d)
+    # 2^-8 the result, 2^-11 a weight, 2^-25 of the largest weight (1) against a weight of e^-score, 2^-19 the exponentials and sums in f32
+    tol = 2.0 ** -8 + 2.0 ** -11 + 2.0 ** -25 * math.exp(score) + 2.0 ** -19
+    assert ((out.double() - want).abs() <= tol * want.abs()).all(), ((out.double() - want).abs() / want).max()
