@@ -304,9 +304,9 @@ __global__ void __launch_bounds__(256) rms_norm_block128_generic_kernel(const No
   }
 }
 
-// silu(g) = g / (1 + e^-g), two at a time, by the hardware's exponential and reciprocal (2^-22 and 1 ulp; 1 + e^-g is never below 1, so
-// neither needs the handling of subnormals that makes their exact forms several instructions each: with those the kernel was
-// instruction-bound, 84 us for 2047 x 28672).  Where e^-g passes the f32 range the result is 0 instead of a number below 2^-121: see tiny().
+// silu(g) = g / (1 + e^-g), two at a time, by the hardware's exponential and reciprocal (2^-22 and 1 ulp; neither needs the handling of
+// subnormals that makes their exact forms several instructions each: with those the kernel was instruction-bound, 84 us for 2047 x 28672).
+// For gates down to kFarGate: the product g log2(e) is rounded, which moves e^-g by |g| 2^-24 of itself, and below -87.3 the reciprocal is 0.
 // silu(g) before u: g * u may overflow where silu(g) is next to 0.
 __device__ __forceinline__ uint64_t silu2(uint64_t g) {
   const uint64_t t = mul2(g, pair(-1.4426950408889634f, -1.4426950408889634f));
@@ -318,11 +318,24 @@ __device__ __forceinline__ uint64_t silu2(uint64_t g) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rb) : "f"(hi(d)));
   return mul2(g, pair(ra, rb));
 }
-// A block this small may be made of results that silu2 has rounded to 0: it is made again by silu_exact, g e^g / (1 + e^g) for negative g.
-__device__ __forceinline__ bool tiny(float amax) { return amax < 7.9e-31f; }   // 2^-100
-__device__ __forceinline__ float silu_exact(float g) {
-  const float e = exp2f(-1.4426950408889634f * fabsf(g));
-  return g * (g < 0.0f ? e : 1.0f) * __frcp_rn(1.0f + e);
+// one element by the same steps
+__device__ __forceinline__ float silu1(float g) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(g, -1.4426950408889634f)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(e, 1.0f)));
+  return __fmul_rn(g, r);
+}
+// Elements whose gate lies below this are made by silu_far: silu(g) u = g e^g u / (1 + e^g), e^g as the square of e^(g/2), so that what g or u is
+// large enough to bring back into range has not been lost before.
+constexpr float kFarGate = -16.0f;
+__device__ __noinline__ float silu_far(float g, float u) {
+  const float e = expf(0.5f * g);
+  return (g * e) * (e * u) / (1.0f + e * e);
+}
+// whether one of eight gates lies below kFarGate (or a pair of them is NaN)
+__device__ __forceinline__ bool far8(const uint4 q) {
+  const __nv_bfloat162* const p = reinterpret_cast<const __nv_bfloat162*>(&q);
+  return !__hbge2(__hmin2(__hmin2(p[0], p[1]), __hmin2(p[2], p[3])), __float2bfloat162_rn(kFarGate));
 }
 
 // A quotient this near to the middle between two E4M3 codes may lie on its other side by the f32 arithmetic in front of it (2^-20 of itself; the
@@ -392,17 +405,23 @@ __global__ void __launch_bounds__(256, 5) swiglu_block128_kernel(const SwigluArg
       unpack8(uq[k], u);
 #pragma unroll
       for (int j = 0; j < 4; ++j) h[k][j] = mul2(silu2(g[j]), u[j]);               // zeros where nothing was loaded
-      amax[k] = max16(absmax8(h[k]));
-      if (__any_sync(0xffffffffu, tiny(amax[k]))) {                                // (a block of zeros comes this way too)
-        if (live[k] && tiny(amax[k])) {
+    }
+    const bool far[2] = {far8(gq[0]), far8(gq[1])};
+    if (__any_sync(0xffffffffu, far[0] || far[1])) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (far[k]) {
           const __nv_bfloat16 *gp = p.gate + row[k] * p.ld + col[k], *up = p.up + row[k] * p.ld + col[k];   // read again: nothing is held for this path
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            h[k][j] = pair(silu_exact(__bfloat162float(gp[2 * j])) * __bfloat162float(up[2 * j]), silu_exact(__bfloat162float(gp[2 * j + 1])) * __bfloat162float(up[2 * j + 1]));
+          for (int j = 0; j < 4; ++j) {
+            const float ga = __bfloat162float(gp[2 * j]), gb = __bfloat162float(gp[2 * j + 1]);
+            h[k][j] = pair(ga < kFarGate ? silu_far(ga, __bfloat162float(up[2 * j])) : lo(h[k][j]),
+                           gb < kFarGate ? silu_far(gb, __bfloat162float(up[2 * j + 1])) : hi(h[k][j]));
+          }
         }
-        amax[k] = max16(absmax8(h[k]));
-      }
     }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) amax[k] = max16(absmax8(h[k]));
     block_scales<2>(amax, F.max_val, mine, inv);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -436,7 +455,8 @@ __global__ void __launch_bounds__(256) swiglu_block128_generic_kernel(const Swig
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t c = b * 128 + j * 32 + lane;
-      h[j] = c < p.cols ? silu_exact(__bfloat162float(p.gate[r * p.ld + c])) * __bfloat162float(p.up[r * p.ld + c]) : 0.0f;
+      const float g = c < p.cols ? __bfloat162float(p.gate[r * p.ld + c]) : 0.0f, u = c < p.cols ? __bfloat162float(p.up[r * p.ld + c]) : 0.0f;
+      h[j] = g < kFarGate ? silu_far(g, u) : __fmul_rn(silu1(g), u);
       amax = fmaxf(amax, fabsf(h[j]));
     }
     const float scale = block_scale(warp_max(amax), F.max_val), inv = __frcp_rn(scale);
