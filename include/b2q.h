@@ -190,11 +190,13 @@ int32_t b2q_rms_norm_quantize_fp8_bf16(b2q_handle h, const void* x_bf16, void* r
 /* b2q_rms_norm_quantize_fp8_bf16 with that scale rule: scale = absmax(y)/max_val per block of 128 columns (1 for a block of
  * zeros, never below 2^-126), code = encode(y/scale).  residual (optional) is updated in place and normalised; y_out (optional)
  * receives bf16(y).  A row that holds a NaN, or whose sum of squares is infinite, gives what the formula gives (NaN, or zeros and
- * NaN); its absmax is taken of the values that are not NaN. */
+ * NaN); its absmax is taken of the values that are not NaN.  The sum of squares of rows that cannot be read 16 bytes at a time (cols % 8 != 0, or
+ * operands off a 16-byte boundary) is taken in another order: scales and y may differ in their last place from those of aligned rows. */
 int32_t b2q_rms_norm_quantize_fp8_block128_bf16(b2q_handle h, const void* x_bf16, void* residual_bf16, const void* gamma_bf16,
                                                 int64_t rows, int64_t cols, float eps, int fmt, int rounding, float* scales,
                                                 uint8_t* codes, void* y_out_bf16);
-/* b2q_swiglu_quantize_rows_bf16 with that scale rule: h = silu(gate) * up in f32, quantized per block of 128 columns. */
+/* b2q_swiglu_quantize_rows_bf16 with that scale rule: h = silu(gate) * up in f32, quantized per block of 128 columns.  E4M3 codes to nearest even
+ * whose f32 quotient lies next to a border between two codes are made again in 64 bits.  Codes and scales do not depend on where the operands lie. */
 int32_t b2q_swiglu_quantize_fp8_block128_bf16(b2q_handle h, const void* gate, const void* up, int64_t rows, int64_t cols,
                                               int64_t ld, int fmt, int rounding, float* scales, uint8_t* codes);
 

@@ -11,8 +11,8 @@
 // instruction-bound).  The norm's quotient is (r' gamma) * (max_val / absmax(r' gamma)): 1 / rms cancels, r' gamma is exact in f32 (two bf16),
 // and the factor is held as a sum of two floats, so that the quotient is rounded once: of 7.4 million codes none differs from the exact
 // quotient's; with each step of the formula rounded 641 did.  SwiGLU multiplies by the reciprocal of the scale, and makes the few elements that
-// come out next to a border between two codes again in 64 bits: 2047 x 28672 takes 58 us instead of 50, and no code above 2^-6 differs where
-// half a code in a million did.
+// come out next to a border between two E4M3 codes again in 64 bits: 2047 x 28672 takes 58 us instead of 50, and of 7.4 million codes above 2^-6
+// none differs from the exact quotient's where half a code in a million did (gates of ordinary size; the window is not a bound of the error).
 #include "common.cuh"
 
 namespace {
@@ -343,30 +343,37 @@ __device__ __forceinline__ bool far8(const uint4 q) {
   return !__hbge2(__hmin2(__hmin2(p[0], p[1]), __hmin2(p[2], p[3])), __float2bfloat162_rn(kFarGate));
 }
 
-// A quotient this near to the middle between two E4M3 codes may lie on its other side by the f32 arithmetic in front of it (2^-20 of itself; the
-// hardware's exponential and reciprocal, and some roundings, are off by about 2^-22 for gates of ordinary size).  Above 2^-6 the middles are the
-// floats whose 20 lowest bits are 0x80000, so the test is one multiply-add and a minimum.
+// A quotient this near to the middle between two E4M3 codes may lie on its other side by the f32 arithmetic in front of it (2^-21 to 2^-20 of
+// itself; the hardware's exponential and reciprocal, and some roundings, are off by about 2^-22 for gates of ordinary size).  Above 2^-6 the middles are
+// the floats whose 20 lowest bits are 0x80000, so the test is one multiply-add and a minimum.
 constexpr uint32_t kNear = 8u << 12;
 __device__ __forceinline__ uint32_t to_middle(float q) { return __float_as_uint(q) * 4096u + (0x80000000u + kNear); }   // below 2 kNear: near
+// The largest of a block between these: its sums have neither over- nor underflowed.
+__device__ __forceinline__ bool in_range(float amax) { return amax >= 0x1p-100f && amax <= 0x1p100f; }
+__device__ __forceinline__ double swiglu64(float g, float u) { return (double)g * (double)u / (1.0 + exp(-(double)g)); }
+__device__ __forceinline__ float quotient64(double h, double top) { return (float)(h * (top > 0.0 ? 448.0 / top : 1.0)); }
 // The codes of a lane's 8 elements by the formula in 64 bits, for a whole warp (blocks of 16 lanes).
 __device__ __noinline__ uint2 swiglu_exact8(const __nv_bfloat16* gp, const __nv_bfloat16* up, bool live) {
   double h[8], top = 0.0;
 #pragma unroll 1
   for (int j = 0; j < 8; ++j) {
-    h[j] = 0.0;
-    if (live) {
-      const double g = (double)__bfloat162float(gp[j]);
-      h[j] = g * (double)__bfloat162float(up[j]) / (1.0 + exp(-g));
-    }
+    h[j] = live ? swiglu64(__bfloat162float(gp[j]), __bfloat162float(up[j])) : 0.0;
     top = fmax(top, fabs(h[j]));
   }
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const double f = top > 0.0 ? 448.0 / top : 1.0;
   uint32_t w[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2((float)(h[2 * j] * f), (float)(h[2 * j + 1] * f)), __NV_SATFINITE, __NV_E4M3);
+  for (int j = 0; j < 4; ++j) w[j] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(quotient64(h[2 * j], top), quotient64(h[2 * j + 1], top)), __NV_SATFINITE, __NV_E4M3);
   return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+}
+// 0xFF in the bytes of those of four quotients that lie near a middle
+__device__ __forceinline__ uint32_t near4(uint64_t a, uint64_t b) {
+  const float q[4] = {lo(a), hi(a), lo(b), hi(b)};
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) m |= to_middle(q[j]) < 2 * kNear ? 0xFFu << (8 * j) : 0u;
+  return m;
 }
 
 struct SwigluArgs {
@@ -437,10 +444,11 @@ __global__ void __launch_bounds__(256, 5) swiglu_block128_kernel(const SwigluArg
         uint32_t near = 0xffffffffu;
 #pragma unroll
         for (int j = 0; j < 4; ++j) near = __vimin3_u32(near, to_middle(lo(q[j])), to_middle(hi(q[j])));
-        const bool sure = amax[k] >= 0x1p-100f && amax[k] <= 0x1p100f;             // of the whole block: its sums have neither over- nor underflowed
-        if (__any_sync(0xffffffffu, live[k] && sure && near < 2 * kNear)) {        // one warp in some two hundred
+        const bool mine = live[k] && in_range(amax[k]) && near < 2 * kNear;
+        if (__any_sync(0xffffffffu, mine)) {                                       // one warp in some two hundred
+          const uint2 m = mine ? make_uint2(near4(q[0], q[1]), near4(q[2], q[3])) : make_uint2(0, 0);
           const uint2 exact = swiglu_exact8(p.gate + row[k] * p.ld + col[k], p.up + row[k] * p.ld + col[k], live[k]);
-          if (sure) codes = exact;
+          codes = make_uint2((exact.x & m.x) | (codes.x & ~m.x), (exact.y & m.y) | (codes.y & ~m.y));
         }
       }
       if (live[k]) *reinterpret_cast<uint2*>(p.codes + row[k] * p.cols + col[k]) = codes;
@@ -448,28 +456,53 @@ __global__ void __launch_bounds__(256, 5) swiglu_block128_kernel(const SwigluArg
   }
 }
 
-// Any length and alignment: one warp per block of 128 columns.
+// Any length and alignment: one warp per block of 128 columns, every element by the steps of the kernel above, so that codes and scales do not
+// depend on where the operands lie.
 __global__ void __launch_bounds__(256) swiglu_block128_generic_kernel(const SwigluArgs p) {
   b2q_pdl_entry();
   const int64_t nb = (p.cols + 127) >> 7, total = p.rows * nb;
   const int lane = threadIdx.x & 31;
   const Fp8Fmt F = fp8_fmt(p.fmt);
+  const bool e4m3_rne = p.fmt == B2Q_FP8_E4M3 && p.rounding == B2Q_ROUND_RNE;
   for (int64_t b0 = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); b0 < total; b0 += (int64_t)gridDim.x * 8) {
     const int64_t r = b0 / nb, b = b0 - r * nb;
-    float h[4], amax = 0.0f;
+    float g[4], u[4], h[4], amax = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t c = b * 128 + j * 32 + lane;
-      const float g = c < p.cols ? __bfloat162float(p.gate[r * p.ld + c]) : 0.0f, u = c < p.cols ? __bfloat162float(p.up[r * p.ld + c]) : 0.0f;
-      h[j] = g < kFarGate ? silu_far(g, u) : __fmul_rn(silu1(g), u);
+      g[j] = c < p.cols ? __bfloat162float(p.gate[r * p.ld + c]) : 0.0f;
+      u[j] = c < p.cols ? __bfloat162float(p.up[r * p.ld + c]) : 0.0f;
+      h[j] = g[j] < kFarGate ? silu_far(g[j], u[j]) : __fmul_rn(silu1(g[j]), u[j]);
       amax = fmaxf(amax, fabsf(h[j]));
     }
-    const float scale = block_scale(warp_max(amax), F.max_val), inv = __frcp_rn(scale);
+    amax = warp_max(amax);
+    const float scale = block_scale(amax, F.max_val), inv = __frcp_rn(scale);
     if (lane == 0) p.scales[b0] = scale;
+    uint32_t code[4];
+    bool near[4], any = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float q = __fmul_rn(h[j], inv);
+      code[j] = encode1(q, p.fmt, p.rounding, F);
+      near[j] = e4m3_rne && in_range(amax) && b * 128 + j * 32 + lane < p.cols && to_middle(q) < 2 * kNear;
+      any |= near[j];
+    }
+    if (__any_sync(0xffffffffu, any)) {
+      double x[4], top = 0.0;
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j) {
+        x[j] = swiglu64(g[j], u[j]);
+        top = fmax(top, fabs(x[j]));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) if (near[j]) code[j] = encode1(quotient64(x[j], top), p.fmt, p.rounding, F);
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t c = b * 128 + j * 32 + lane;
-      if (c < p.cols) p.codes[r * p.cols + c] = (uint8_t)encode1(__fmul_rn(h[j], inv), p.fmt, p.rounding, F);
+      if (c < p.cols) p.codes[r * p.cols + c] = (uint8_t)code[j];
     }
   }
 }
