@@ -238,22 +238,32 @@ class QuantizedLlamaRunner:
         xc, xs = rms_norm_quantize_fp8(delta, self.g_final, cfg.eps, residual=res)
         return xc, xs
 
+    def _cache_batch(self, seqs):
+        """The batch as the cache reads it (lengths, block tables, row offsets): one upload each, nothing is read back.  Of a table the blocks that
+        the sequence fills are taken; what stands behind them is not looked at."""
+        cfg = self.cfg
+        tables = []
+        for r0, r1, p0, table in seqs:
+            need = -(-(p0 + r1 - r0) // cfg.block_size)
+            if need > len(table):
+                raise L.DimensionMismatch(L.ERR_DIMENSION_MISMATCH, f"expected {need} KV blocks, got {len(table)}")
+            used = list(table[:need])
+            if any(not 0 <= b < cfg.num_blocks for b in used):
+                raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, f"block table {used} names a block outside [0, {cfg.num_blocks})")
+            tables.append(used)
+        width = max(1, max(len(t) for t in tables))
+        lens = torch.tensor([p0 + r1 - r0 for r0, r1, p0, _ in seqs], dtype=torch.int32, device=self.dev)
+        tables = torch.tensor([t + [-1] * (width - len(t)) for t in tables], dtype=torch.int32, device=self.dev)
+        single = all(r1 - r0 == 1 for r0, r1, _, _ in seqs)
+        starts = None if single else torch.tensor([r0 for r0, _, _, _ in seqs] + [seqs[-1][1]], dtype=torch.int32, device=self.dev)
+        return lens, tables, starts
+
     def _forward_block128(self, token_ids: torch.Tensor, positions: torch.Tensor, seqs):
         cfg = self.cfg
         tokens, nq, nkv, d = token_ids.numel(), cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
         delta = self.embed[token_ids.long()].contiguous()
         res = torch.zeros(tokens, cfg.hidden, dtype=torch.bfloat16, device=self.dev)
-        # the batch as the cache reads it: one upload each, nothing is read back
-        for r0, r1, p0, table in seqs:
-            if -(-(p0 + r1 - r0) // cfg.block_size) > len(table):
-                raise L.DimensionMismatch(L.ERR_DIMENSION_MISMATCH, f"expected {-(-(p0 + r1 - r0) // cfg.block_size)} KV blocks, got {len(table)}")
-            if any(not 0 <= b < cfg.num_blocks for b in table):
-                raise L.InvalidArgument(L.ERR_INVALID_ARGUMENT, f"block table {list(table)} names a block outside [0, {cfg.num_blocks})")
-        width = max(1, max(len(t) for _, _, _, t in seqs))
-        lens = torch.tensor([p0 + r1 - r0 for r0, r1, p0, _ in seqs], dtype=torch.int32, device=self.dev)
-        tables = torch.tensor([list(t) + [-1] * (width - len(t)) for _, _, _, t in seqs], dtype=torch.int32, device=self.dev)
-        single = all(r1 - r0 == 1 for r0, r1, _, _ in seqs)
-        starts = None if single else torch.tensor([r0 for r0, _, _, _ in seqs] + [seqs[-1][1]], dtype=torch.int32, device=self.dev)
+        lens, tables, starts = self._cache_batch(seqs)
         for layer in self.layers:
             x_in = delta
             xc, xs = rms_norm_quantize_fp8_block128(delta, layer.g_attn, cfg.eps, residual=res)

@@ -57,3 +57,21 @@ def test_contiguous_weights_stay_static(recorded):
     h = recorded(Recorder())
     blas.gemm_fp8_block128(*_operands(None))
     assert h.seen == [("b2q_gemm_fp8_block128", True)]
+
+
+def test_runner_reads_the_blocks_that_a_sequence_fills(libb2q):
+    """Block tables come padded: what stands behind the blocks in use is neither refused nor uploaded."""
+    from oxicuda_b200 import _lib
+    from oxicuda_b200.model_runner import LlamaConfig, QuantizedLlamaRunner
+    runner = object.__new__(QuantizedLlamaRunner)
+    runner.cfg, runner.dev = LlamaConfig(recipe="block128", block_size=16, num_blocks=64), "cpu"
+    lens, tables, starts = runner._cache_batch([(0, 1, 15, [3, -1, -1, -1]), (1, 2, 16, [5, 63, 64, 1 << 40])])
+    assert lens.tolist() == [16, 17] and tables.tolist() == [[3, -1], [5, 63]] and starts is None
+    lens, tables, starts = runner._cache_batch([(0, 40, 0, (7, 8, 9, -1)), (40, 41, 0, [1])])
+    assert lens.tolist() == [40, 1] and tables.tolist() == [[7, 8, 9], [1, -1, -1]] and starts.tolist() == [0, 40, 41]
+    with pytest.raises(_lib.InvalidArgument):
+        runner._cache_batch([(0, 1, 16, [3, -1])])
+    with pytest.raises(_lib.InvalidArgument):
+        runner._cache_batch([(0, 1, 16, [3, 64])])
+    with pytest.raises(_lib.DimensionMismatch):
+        runner._cache_batch([(0, 1, 16, [3])])

@@ -158,3 +158,15 @@ def test_runner_contract_and_refusals(cuda):
             QuantizedLlamaRunner(bad, cuda)
     with pytest.raises(_lib.UnsupportedOperation):
         QuantizedLlamaRunner(LlamaConfig(recipe="block128", block_size=24), cuda)
+
+
+def test_padded_block_tables(cuda):
+    """Tables as a server keeps them, padded to one width, give the logits of exact ones."""
+    from oxicuda_b200.model_runner import LlamaConfig, QuantizedLlamaRunner
+    cfg = LlamaConfig(n_layers=1, recipe="block128")
+    got = []
+    for pad in ([], [-1] * 9):
+        runner = QuantizedLlamaRunner(cfg, cuda, seed=4)
+        tables = [[9, 1, 3] + pad, [2, 30] + pad]
+        got.append([runner.prefill(list(range(40)), [0, 33, 40], tables), runner.decode([5, 6], tables, [33, 7])])
+    assert got[0] == got[1]
