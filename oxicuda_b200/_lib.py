@@ -270,15 +270,17 @@ class Handle:
         if st != OK:
             msg = lib().b2q_last_error(self._h)
             raise _ERRORS.get(st, B2qError)(st, msg.decode() if msg else name)
+        if name == "b2q_set_stream":              # what is kept of the handle's state follows it, whoever sets it
+            self._stream = getattr(args[0], "value", args[0]) or 0
+        elif name == "b2q_set_static_weights":
+            self.static_weights = bool(getattr(args[0], "value", args[0]))
 
     def set_stream(self, stream_ptr: int):
         self.call("b2q_set_stream", C.c_void_p(stream_ptr))
-        self._stream = stream_ptr
 
     def set_static_weights(self, static_weights: bool):
         """False: weight operands may be produced by the kernel right before a call (see include/b2q.h)."""
         self.call("b2q_set_static_weights", 1 if static_weights else 0)
-        self.static_weights = bool(static_weights)
 
     def sm_version(self) -> int:
         v = _I()

@@ -75,3 +75,42 @@ def test_runner_reads_the_blocks_that_a_sequence_fills(libb2q):
         runner._cache_batch([(0, 1, 16, [3, 64])])
     with pytest.raises(_lib.DimensionMismatch):
         runner._cache_batch([(0, 1, 16, [3])])
+
+
+def test_a_handle_knows_the_stream_that_was_set_by_its_entry_point(libb2q, monkeypatch):
+    """default_handle() sets a handle's stream only where it is another one than the handle launches on: a stream set through call() counts."""
+    import ctypes as C
+    from oxicuda_b200 import _lib
+
+    class Library:
+        def __init__(self):
+            self.streams, self.static = [], None
+
+        def b2q_set_stream(self, h, stream):
+            self.streams.append(getattr(stream, "value", stream) or 0)
+            return 0
+
+        def b2q_set_static_weights(self, h, on):
+            self.static = bool(on)
+            return 0
+
+    lib = Library()
+    h = object.__new__(_lib.Handle)
+    h._h, h._stream, h.static_weights, h.device = None, 0, True, 0
+    monkeypatch.setattr(_lib, "_lib", lib)
+    monkeypatch.setattr(_lib, "_default", {0: h})
+    now = [0x10]
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: now[0], raising=False)
+    assert _lib.default_handle(0) is h and lib.streams == [0x10]
+    _lib.default_handle(0)
+    assert lib.streams == [0x10]
+    for other in (C.c_void_p(0x20), 0x30, None):
+        h.call("b2q_set_stream", other)
+        _lib.default_handle(0)
+        assert lib.streams[-1] == 0x10
+    now[0] = 0
+    h.call("b2q_set_stream", None)
+    _lib.default_handle(0)
+    assert lib.streams[-1] == 0
+    h.call("b2q_set_static_weights", 0)
+    assert not h.static_weights and lib.static is False
