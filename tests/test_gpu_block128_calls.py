@@ -47,3 +47,25 @@ def test_weights_written_right_before_the_product(cuda, M):
     finally:
         h.set_static_weights(True)
     h.check()
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("fmt", [0, 1])
+def test_scales_of_every_block(cuda, block_rows, fmt):
+    """quantize_fp8_blocks: every block's scale is its own absmax / max_val (1 for zeros), short blocks at the edges included."""
+    from oxicuda_b200.quant import quantize_fp8_blocks
+    g = torch.Generator(device=cuda).manual_seed(3)
+    for dtype in (torch.float32, torch.bfloat16):
+        for rows, cols in ((256, 384), (130, 200), (1, 1)):
+            x = (torch.randn(rows, cols, device=cuda, generator=g) * torch.exp(3 * torch.randn(rows, 1, device=cuda, generator=g))).to(dtype)
+            if cols > 128:
+                x[:128, :128] = 0
+            codes, scales = quantize_fp8_blocks(x, block_rows, fmt=fmt)
+            rb, cb = -(-rows // block_rows), -(-cols // 128)
+            b = torch.nn.functional.pad(x.double(), (0, cb * 128 - cols, 0, rb * block_rows - rows)).view(rb, block_rows, cb, 128)
+            top = b.abs().amax(dim=(1, 3))
+            want = torch.where(top > 0, top / (448.0, 57344.0)[fmt], torch.ones_like(top))
+            assert scales.shape == (rb, cb) and ((scales.double() - want).abs() <= 2.0 ** -23 * want).all()   # a division in f32: half a step
+            # the largest element of a block is the largest code: its quotient is max_val but for two roundings, 2^-23 of it
+            full = torch.nn.functional.pad(codes, (0, cb * 128 - cols, 0, rb * block_rows - rows)).view(rb, block_rows, cb, 128) & 127
+            assert (full.amax(dim=(1, 3)) == torch.where(top > 0, (126, 123)[fmt], 0)).all()

@@ -125,3 +125,36 @@ def test_small_weights_on_pages_of_a_smaller_scale(cuda, new, top, lead, low, sc
     # 2^-8 the result, 2^-11 a weight, 2^-25 of the largest weight (1) against a weight of e^-score, 2^-19 the exponentials and sums in f32
     tol = 2.0 ** -8 + 2.0 ** -11 + 2.0 ** -25 * math.exp(score) + 2.0 ** -19
     assert ((out.double() - want).abs() <= tol * want.abs()).all(), ((out.double() - want).abs() / want).max()
+
+
+def test_rows_beside_a_bad_page_are_right(cuda):
+    """A table entry that names no page is left out of its own sequence, with and without row offsets; the others come out as they should."""
+    from oxicuda_b200 import _lib as L
+    from tests.test_gpu_kv8 import _check as check, _pages, _q
+    for new in (1, 3, 40):
+        lens = [40, 50, 60, 70]
+        cache, table = _pages(cuda, lens, 16, 2, 128, 14)
+        q = _q(cuda, 4 * new, 8, 128, 3)
+        seq = torch.tensor(lens, dtype=torch.int32, device=cuda)
+        bad = table.clone()
+        bad[0, 1], bad[3, 0] = cache.num_pages, -5
+        for starts in ((None,) if new == 1 else ()) + (torch.arange(0, 4 * new + 1, new, dtype=torch.int32, device=cuda),):
+            out = cache.attend(q, seq, bad, q_starts=starts)
+            with pytest.raises(L.InvalidArgument):
+                L.default_handle().check()
+            assert torch.isfinite(out).all()
+            check(cache, table[1:3], lens[1:3], [new, new], q[new: 3 * new], out[new: 3 * new])
+            # the keys of the pages that are there, by definition
+            pos = lens[0] - new + torch.arange(new, device=cuda)
+            j = torch.tensor([i for i in range(lens[0]) if i // 16 != 1], device=cuda)
+            for h in range(2):
+                pages = table[0, j // 16].long()
+                k, v = [c[pages, h, j % 16].view(torch.float8_e4m3fn).double() * torch.exp2(s[pages, h].double() - 127)[:, None]
+                        for c, s in ((cache.k_codes, cache.k_scales), (cache.v_codes, cache.v_scales))]
+                qq = q[:new, 4 * h: 4 * h + 4].double()
+                s = (torch.einsum("qgd,kd->gqk", qq, k) * 128 ** -0.5).masked_fill(~(j[None] <= pos[:, None])[None], float("-inf"))
+                p = torch.softmax(s, dim=2)
+                want, A = torch.einsum("gqk,kd->qgd", p, v), torch.einsum("gqk,kd->qgd", p, v.abs())
+                delta = 128 ** -0.5 * qq.abs().amax(dim=2) * k.abs().sum(dim=1).amax() * (2.0 ** -17 + 2.0 ** -16)
+                err = (out[:new, 4 * h: 4 * h + 4].double() - want).abs()
+                assert (err <= 2.0 ** -8 * want.abs() + (2.0 ** -11 + 3 * delta[..., None]) * A + 2.0 ** -17 * v.abs().sum(dim=0)).all()
