@@ -318,7 +318,7 @@ class PagedFp8KvCache:
         """Causal attention of q (bf16 [tokens, heads, head_dim], heads a multiple of n_kv_heads) over the cached tokens, the rows' own
         included; with window > 0 over the last `window` of them.  scale: 1 / sqrt(head_dim) unless given.  Returns out (bf16, q's shape)
         and, when asked, the log-sum-exp of the scores (f32 [tokens, heads]).  Rows outside every sequence are left as they were (`out`
-        given) or unspecified."""
+        given) or unspecified.  `out` may be q itself, and overlaps nothing else that the call reads."""
         q, ld_q = self._rows("attend", q, 0)
         tokens, heads, d = q.shape
         if heads == 0 or heads % self.n_kv_heads != 0:

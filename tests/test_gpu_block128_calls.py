@@ -69,3 +69,18 @@ def test_scales_of_every_block(cuda, block_rows, fmt):
             # the largest element of a block is the largest code: its quotient is max_val but for two roundings, 2^-23 of it
             full = torch.nn.functional.pad(codes, (0, cb * 128 - cols, 0, rb * block_rows - rows)).view(rb, block_rows, cb, 128) & 127
             assert (full.amax(dim=(1, 3)) == torch.where(top > 0, (126, 123)[fmt], 0)).all()
+
+
+@pytest.mark.parametrize("new,old,heads", [(1, 9000, 8), (1, 50, 80), (4, 3000, 8), (150, 0, 8), (40, 9000, 8)])
+def test_attention_over_its_own_queries(cuda, new, old, heads):
+    """out may be q itself: every CTA of a row tile has read its rows before one of them writes."""
+    from tests.test_gpu_kv8 import _pages, _q
+    lens = [old + new, new + 7]
+    cache, table = _pages(cuda, lens, 32, 2, 128, new)
+    q = _q(cuda, 2 * new, heads, 128, new)
+    seq = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    starts = None if new == 1 else torch.tensor([0, new, 2 * new], dtype=torch.int32, device=cuda)
+    want = cache.attend(q, seq, table, q_starts=starts)
+    for _ in range(5):
+        x = q.clone()
+        assert cache.attend(x, seq, table, q_starts=starts, out=x) is x and torch.equal(x, want)
