@@ -97,8 +97,8 @@ constexpr int kSpan = 8, kDrop = 64;
 constexpr int kLeast = -40;
 // what outputs are multiplied by when R moves: 2^(from - to), exact down to 2^-149 and 0 below (R may rise by 2^171)
 __device__ __forceinline__ float move_unit(int from, int to) {
-  const int d = from - to;
-  return d >= -126 ? pow2i(d) : d >= -149 ? __uint_as_float(1u << (d + 149)) : 0.0f;
+  const int d = max(from - to, -150);              // at most kDrop
+  return __uint_as_float(d >= -126 ? (uint32_t)(d + 127) << 23 : (1u << (d + 150)) >> 1);
 }
 // R for pages whose value scales lie from 2^least to 2^lead, lead + room - least at most kSpan; `top` is the largest R so far.  Returns what outputs are
 // to be multiplied by.
