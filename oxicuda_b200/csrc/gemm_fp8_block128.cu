@@ -7,9 +7,11 @@
 // scale changes with every block of 128 along K, so each block's product is a fresh TMEM accumulator (512 / BN of them in
 // flight), and eight epilogue warps per CTA add scale * product to sums that they hold in registers (BN / 2 columns of one row
 // per thread) while the tensor core works on the next blocks.  Per block and CTA the tensor core needs 128 x BN x 128 / 8192 =
-// 2 BN clocks; the epilogue reads BN columns of TMEM and issues BN / 2 two-wide FMAs per warp scheduler, which fits beside it.
-// Measured: 4096 x 8192 x 28672 831 to 853 us (2.3 PFLOP/s, two thirds of the FP8 rate; the power cap acts), 2048 x 8192 x 8192 127 us (2.2),
-// 512 x 8192 x 8192 35 us (1.9).
+// 2 BN clocks; the epilogue reads BN columns of TMEM and issues BN / 2 two-wide FMAs per warp scheduler, which fits beside it in issue slots, but not in
+// time: a thread reads 16 columns, waits for them, adds, and reads the next.
+// Measured: 4096 x 8192 x 28672 835 to 845 us in a graph of eight (2.3 PFLOP/s), 950 in runs long enough for the power cap (2.0; a call among others
+// 986), 2048 x 8192 x 8192 130 us (2.1), 512 x 8192 x 8192 36 us (1.9).  The read-out bounds it: the product with a scale per row, whose accumulators
+// are read once a tile, takes 670 us (745) at the first shape; at 4096 x 8192 x 8192 the tensor pipe is active 61 % of the time here and 88 % there.
 #include "tc_common.cuh"
 
 namespace b128 {

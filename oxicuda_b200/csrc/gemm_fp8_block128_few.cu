@@ -7,8 +7,8 @@
 //     to sums in registers.
 //   * Two CTAs share an SM up to 64 tokens, so that one streams weights while the other starts or ends (a ring of about 100 KiB each).
 //   * Programmatic dependent launch: with static weights the weight copies start before the previous kernel of the stream has ended.
-// Bound by HBM.  Measured back to back over rotating weights: 16 x 8192 x 28672 38 us (6.2 TB/s), 64 x 8192 x 28672 41 us (5.7), 53 x 10240 x 8192
-// 19.6 us (4.4: 240 CTAs on 296 places), 1 x 14336 x 4096 12.6 us (4.7: launch and ramp).
+// Bound by HBM.  Measured back to back over rotating weights: 16 x 8192 x 28672 38 us (6.1 TB/s), 64 x 8192 x 28672 42 us (5.7), 53 x 10240 x 8192
+// 20.4 us (4.2: 240 CTAs on 148 SMs, some with one of them and some with two), 1 x 14336 x 4096 13.1 us (4.5: 224 CTAs, launch and ramp).
 // Every mbarrier wait is bounded; on expiry the kernel records B2Q_ERR_TIMEOUT and leaves.
 #include "tc_common.cuh"
 #include <cooperative_groups.h>

@@ -20,7 +20,7 @@
 // one after the other.
 // Keys behind the last visible one are masked and their value rows zeroed before they are multiplied, so stale codes cannot reach a
 // result; a page that the table does not name is neither read nor counted.
-// Measured: 32 sequences x 8200 keys (32 heads of 128 channels over 8 kv heads) 90 us, 4.5 TB/s of cache (pages of 16: 94 us); the same copies
+// Measured: 32 sequences x 8200 keys (32 heads of 128 channels over 8 kv heads) 88 us, 4.6 TB/s of cache (pages of 16: 94 us); the same copies
 // without the arithmetic 74 us.  256 equal CTAs share 148 SMs there, so the SMs that hold two set the time.
 // Every mbarrier wait is bounded; on expiry the kernel records B2Q_ERR_TIMEOUT and leaves.
 #include "kv8.cuh"

@@ -12,8 +12,8 @@
 // Work per 64 keys and CTA: 640 clocks of tensor core (Q K^T at N = 64 reads 1.5 x the shared memory that its rate allows, P V at N = D
 // runs at rate), 512 of exponentials and 120 KB of shared memory traffic (48 for Q K^T, 16 for P V, 40 to convert the values, 16 to bring the
 // tiles in), 940 clocks: two CTAs share an SM, so that one multiplies while the other exponentiates.
-// Measured: 2 x 3900 tokens behind 150 (32 heads of 128 channels over 8 kv heads) 283 us, 765 TFLOP/s; 1 x 8000 tokens 523 us, 1000 TFLOP/s,
-// where a tile takes about 1100 clocks.  Leaving out the exponentials changes nothing there, leaving out the conversion of the values saves 6 %,
+// Measured in a graph of eight: 2 x 3900 tokens behind 150 (32 heads of 128 channels over 8 kv heads) 277 us, 780 TFLOP/s (a call among others 308;
+// pages of 16 292 to 319); 1 x 8000 tokens 522 us, 1000 TFLOP/s, where a tile takes about 1100 clocks.  Leaving out the exponentials changes nothing there, leaving out the conversion of the values saves 6 %,
 // three quarters of Q K^T 10 %: shared memory bounds it, with the products' latency on top in short rows.
 // The running maximum is followed lazily: it moves only when a score exceeds it by more than 2^kSlack (f16 has the range), so O is rescaled
 // (a round trip through registers) once or twice per row and not per tile.  The value scale of a page is a power of two 2^lv: weights
