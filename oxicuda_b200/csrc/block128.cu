@@ -11,8 +11,9 @@
 // instruction-bound).  The norm's quotient is (r' gamma) * (max_val / absmax(r' gamma)): 1 / rms cancels, r' gamma is exact in f32 (two bf16),
 // and the factor is held as a sum of two floats, so that the quotient is rounded once: of 7.4 million codes none differs from the exact
 // quotient's; with each step of the formula rounded 641 did.  SwiGLU multiplies by the reciprocal of the scale, and makes the few elements that
-// come out next to a border between two E4M3 codes again in 64 bits: 2047 x 28672 takes 58 us instead of 50 over one set of inputs (65 a call), and of 7.4 million codes above 2^-6
-// none differs from the exact quotient's where half a code in a million did (gates of ordinary size; the window is not a bound of the error).
+// come out next to a border between two E4M3 codes again in 64 bits: 2047 x 28672 takes 58 us instead of 50 over one set of inputs (65 a call), and
+// of 7.4 million codes above 2^-6 none differs from the exact quotient's where half a code in a million did (gates of ordinary size; the window is
+// no bound of the error).
 #include "common.cuh"
 
 namespace {
