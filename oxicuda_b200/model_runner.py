@@ -87,6 +87,8 @@ class LlamaConfig:
             raise L.InvalidConfig(L.ERR_INVALID_CONFIG, f"recipe must be per_token or block128, got {self.recipe!r}")
         if self.recipe == "block128" and (self.n_heads * self.head_dim) % 128 != 0:
             raise L.InvalidConfig(L.ERR_INVALID_CONFIG, f"block128: n_heads * head_dim must be a multiple of 128, got {self.n_heads * self.head_dim}")
+        if self.recipe == "block128" and self.kv_bits != 8:
+            raise L.InvalidConfig(L.ERR_INVALID_CONFIG, f"block128: the paged E4M3 cache holds 8 bits, got kv_bits={self.kv_bits}")
 
 
 class Fp8Block128Linear:

@@ -114,3 +114,13 @@ def test_a_handle_knows_the_stream_that_was_set_by_its_entry_point(libb2q, monke
     assert lib.streams[-1] == 0
     h.call("b2q_set_static_weights", 0)
     assert not h.static_weights and lib.static is False
+
+
+def test_a_width_that_the_cache_does_not_have_is_refused(libb2q):
+    from oxicuda_b200 import _lib
+    from oxicuda_b200.model_runner import LlamaConfig
+    LlamaConfig(kv_bits=4).validate()
+    LlamaConfig(recipe="block128", kv_bits=8).validate()
+    for bits in (2, 4, 16):
+        with pytest.raises(_lib.InvalidConfig):
+            LlamaConfig(recipe="block128", kv_bits=bits).validate()
